@@ -45,6 +45,12 @@ enum {
   HCU_DTYPE_BF16 = 1,
 };
 
+/* MLA cache slot formats (layouts at hcu_rope_qout_kv_store / hcu_store_mla_kv4). */
+enum {
+  HCU_KV_FP8_656 = 0, /* 656-byte slot: fp8 latent, fp32 group scales, bf16 rope */
+  HCU_KV_FP4_432 = 1, /* 432-byte slot: 4-bit latent, e4m3 group scales, fp32 token scale, bf16 rope */
+};
+
 /* Device status bits (sticky until cleared). */
 enum {
   HCU_STATUS_WAIT_TIMEOUT = 1u << 0, /* an mbarrier / flag wait hit its bound */
@@ -418,6 +424,91 @@ int hcu_topk_keys_if(const float* score, int64_t rows, int64_t width, int64_t sc
                      const int16_t* mask, int64_t mask_stride, const int32_t* lengths,
                      const int32_t* page_table, int64_t pt_stride, int32_t* dst, uint32_t* dst_keys,
                      const int32_t* run_if, hcu_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Sparse attention around the indexer (no counterpart among the reference's
+ * sources: its allocator, tables and sparse attention are sglang's and closed
+ * libraries').  The tables of a step, the blocks or tokens a row attends to, a
+ * 4-bit form of the MLA slot, and the attention over either slot format.
+ * ------------------------------------------------------------------------ */
+
+/* Tables of one step from the requests' lengths, and the pages its new tokens
+ * take, in one launch.
+ *   req_pages  int32 [n_req, max_pages] row stride req_stride: each request's page
+ *              ids; the pages taken in this step are written in place
+ *   req_idx / seq_lens / new_lens  int32 [batch]: the request's row in req_pages
+ *              (no row twice), its cached tokens, its new tokens of this step
+ *   free_pages int32 [n_free]: page ids handed out in order from free_head[0]
+ *   n_rows     query rows of the outputs: the new tokens, request by request; rows
+ *              past sum(new_lens) are written as empty (length 0, entries -1)
+ *   width      tokens per row of page_table, a multiple of 64
+ *   block_table int32 [n_rows, width / 64], page_table int32 [n_rows, width]
+ *              (16-byte aligned): page ids and slots page * 64 + offset of the
+ *              request's seq + new tokens (every row of a request alike), -1 after
+ *   lengths    int32 [n_rows]: visible tokens, position + 1 (at most width)
+ *   positions  int32 [n_rows]; token_loc int32 / loc int64 [n_rows]: the new
+ *              token's slot, -1 where the free pages ran out
+ *   free_head_out int32 [1]: free_head[0] + pages taken (must not alias free_head)
+ * Sets HCU_STATUS_BAD_INPUT when free pages run out, a request outgrows max_pages
+ * or width, a length is negative, a request row is out of range, or sum(new_lens)
+ * exceeds n_rows; nothing is read or written out of range. */
+int hcu_step_tables(int32_t* req_pages, int64_t n_req, int64_t max_pages, int64_t req_stride,
+                    const int32_t* req_idx, const int32_t* seq_lens, const int32_t* new_lens, int64_t batch,
+                    const int32_t* free_pages, int64_t n_free, const int32_t* free_head, int64_t n_rows,
+                    int64_t width, int32_t* block_table, int32_t* page_table, int32_t* lengths,
+                    int32_t* positions, int32_t* token_loc, int64_t* loc, int32_t* free_head_out,
+                    hcu_stream_t stream);
+
+/* The n_blocks 64-token blocks of each row with the largest scores, a block's
+ * score being the largest of its visible tokens' (score where the mask bit is
+ * set, else +0); ties to the lower block.  The first n_sink and the last n_local
+ * visible blocks are always among them (n_sink + n_local <= n_blocks).
+ *   score / mask / lengths as hcu_sparse_mask_topk_transform (score 16-byte aligned,
+ *   score_stride % 4 == 0); width up to 3145728
+ *   out int32 [rows, n_blocks]: block indices in ascending order, -1 pads */
+int hcu_select_blocks(const float* score, int64_t rows, int64_t width, int64_t score_stride,
+                      const int16_t* mask, int64_t mask_stride, const int32_t* lengths, int64_t n_blocks,
+                      int64_t n_sink, int64_t n_local, int32_t* out, hcu_stream_t stream);
+
+/* 4-bit MLA slot writer.  Slot (432 bytes): 512 e2m1 codes (element 2j in the low
+ * half of byte j) | 32 e4m3 scales of 16 elements | fp32 token scale | 12 zero
+ * bytes | 64 bf16 rope.  t = 2^(floor(log2(amax)) - 10) (at least 2^-100),
+ * sg = e4m3(amax_g / (6 t)), code = e2m1(x / (sg t)), all round to nearest even
+ * and saturated; an element stands for code * sg * t.
+ *   kv_c  bf16 [n_tokens, 512] row stride kv_tok (16-byte aligned rows), finite
+ *   k_pe  bf16 [n_tokens, 64] row stride k_tok (rotated rope, copied)
+ *   loc   int64 [n_tokens]; slots out of range are skipped and flagged */
+int hcu_store_mla_kv4(const uint16_t* kv_c, int64_t kv_tok, const uint16_t* k_pe, int64_t k_tok, const int64_t* loc,
+                      int64_t n_tokens, uint8_t* kv_buffer, int64_t n_slots, int64_t slot_stride,
+                      hcu_stream_t stream);
+
+/* hcu_dequant_k_cache_paged for the 432-byte slot: out bf16 [n_tokens, 576] (exact
+ * values). */
+int hcu_dequant_mla_kv4_paged(const uint8_t* kv_buffer, int64_t n_slots, int64_t slot_stride,
+                              const int32_t* page_table_1, int64_t n_tokens, uint16_t* out, hcu_stream_t stream);
+
+/* MLA attention over selected tokens: with k[t] the 576 values of slot t (512
+ * latent, 64 rope), s[h, t] = sm_scale * q[h] . k[t], out[h] = softmax(s[h]) .
+ * k[:, :512] and lse[h] = log sum_t exp(s[h, t]) over the row's tokens.
+ *   q        bf16 [rows, heads, 576], strides q_row / q_head (multiples of 8), 16-byte aligned
+ *   kv_cache uint8 [n_slots, slot_stride] in kv_format (HCU_KV_*)
+ *   token form (block_table null): indices int32 [rows, n_idx] slots, negative entries
+ *            skipped (what hcu_sparse_mask_topk_transform writes)
+ *   block form: indices int32 [rows, n_idx] blocks of the row (what hcu_select_blocks
+ *            writes, negative entries skipped); block b is page block_table[row, b]
+ *            (int32 [rows, n_bt]) and its tokens at positions below lengths[row] count
+ *   out bf16 [rows, heads, 512], lse fp32 [rows, heads]; a row without tokens gives
+ *            out 0 and lse -inf
+ *   workspace >= hcu_sparse_mla_attention_workspace_bytes(rows, heads, n_idx tokens: n_idx
+ *            or 64 * n_idx), 256-byte aligned, no initial contents needed
+ * Slots or blocks out of range are skipped and flagged HCU_STATUS_BAD_INPUT. */
+int64_t hcu_sparse_mla_attention_workspace_bytes(int64_t rows, int64_t heads, int64_t n_tokens);
+int hcu_sparse_mla_attention(const uint16_t* q, int64_t rows, int64_t heads, int64_t q_row, int64_t q_head,
+                             const uint8_t* kv_cache, int64_t n_slots, int64_t slot_stride, int32_t kv_format,
+                             const int32_t* indices, int64_t n_idx, int64_t idx_stride, const int32_t* block_table,
+                             int64_t bt_stride, int64_t n_bt, const int32_t* lengths, float sm_scale,
+                             void* workspace, int64_t workspace_bytes, uint16_t* out, float* lse,
+                             hcu_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -561,6 +561,157 @@ std::vector<torch::Tensor> topk_keys_if(const torch::Tensor& score, const torch:
   return {dst, keys};
 }
 
+// ------------------------------------------------------- sparse attention around the indexer
+std::vector<torch::Tensor> step_tables(torch::Tensor& req_pages, const torch::Tensor& req_idx,
+                                       const torch::Tensor& seq_lens, const torch::Tensor& new_lens,
+                                       const torch::Tensor& free_pages, const torch::Tensor& free_head, int64_t n_rows,
+                                       int64_t width) {
+  TORCH_CHECK(req_pages.is_cuda() && req_pages.scalar_type() == at::kInt && req_pages.dim() == 2 &&
+                  (req_pages.numel() == 0 || req_pages.stride(1) == 1) && req_pages.stride(0) >= req_pages.size(1),
+              "req_pages must be a row-contiguous int32 CUDA tensor [requests, pages]");
+  const int64_t B = req_idx.size(0);
+  const auto vec = [&](const torch::Tensor& t, int64_t n) {
+    return t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && t.size(0) == n &&
+           t.device() == req_pages.device();
+  };
+  TORCH_CHECK(vec(req_idx, B) && vec(seq_lens, B) && vec(new_lens, B),
+              "req_idx, seq_lens and new_lens must be contiguous int32 [batch] on req_pages' device");
+  TORCH_CHECK(vec(free_pages, free_pages.numel()) && vec(free_head, 1),
+              "free_pages and free_head must be contiguous int32 [n] and [1] on req_pages' device");
+  TORCH_CHECK(n_rows >= 0 && width > 0 && width % 64 == 0, "width must be a positive multiple of 64, n_rows >= 0");
+  const c10::cuda::CUDAGuard guard(req_pages.device());
+  const auto i32 = req_pages.options();
+  auto bt = torch::empty({n_rows, width / 64}, i32);
+  auto pt = torch::empty({n_rows, width}, i32);
+  auto len = torch::empty({n_rows}, i32);
+  auto pos = torch::empty({n_rows}, i32);
+  auto tl = torch::empty({n_rows}, i32);
+  auto loc = torch::empty({n_rows}, i32.dtype(at::kLong));
+  auto head = torch::empty({1}, i32);
+  check_status(hcu_step_tables(ptr<int32_t>(req_pages), req_pages.size(0), req_pages.size(1), req_pages.stride(0),
+                               ptr<const int32_t>(req_idx), ptr<const int32_t>(seq_lens), ptr<const int32_t>(new_lens),
+                               B, ptr<const int32_t>(free_pages), free_pages.size(0), ptr<const int32_t>(free_head),
+                               n_rows, width, ptr<int32_t>(bt), ptr<int32_t>(pt), ptr<int32_t>(len), ptr<int32_t>(pos),
+                               ptr<int32_t>(tl), ptr<int64_t>(loc), ptr<int32_t>(head), cur_stream()),
+               "step_tables");
+  return {bt, pt, len, pos, tl, loc, head};
+}
+
+torch::Tensor select_blocks(const torch::Tensor& score, const torch::Tensor& nonzero_mask, const torch::Tensor& lengths,
+                            int64_t n_blocks, int64_t n_sink, int64_t n_local) {
+  TORCH_CHECK(score.is_cuda() && score.scalar_type() == at::kFloat && score.dim() == 2 &&
+                  (score.numel() == 0 || score.stride(1) == 1) && score.stride(0) % 4 == 0 &&
+                  score.stride(0) >= score.size(1),
+              "score must be row-contiguous float32 [rows, width] with a row stride that is a multiple of 4");
+  const int64_t rows = score.size(0);
+  TORCH_CHECK(nonzero_mask.scalar_type() == at::kShort && nonzero_mask.dim() == 2 &&
+                  (nonzero_mask.numel() == 0 || nonzero_mask.stride(1) == 1) && nonzero_mask.size(0) == rows &&
+                  nonzero_mask.size(1) == (score.size(1) + 15) / 16,
+              "nonzero_mask must be row-contiguous int16 [rows, ceil(width/16)]");
+  TORCH_CHECK(lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.is_contiguous() &&
+                  lengths.size(0) == rows,
+              "lengths must be contiguous int32 [rows]");
+  TORCH_CHECK(nonzero_mask.device() == score.device() && lengths.device() == score.device(),
+              "all tensors must be on the score's device");
+  TORCH_CHECK(n_blocks >= 1 && n_sink >= 0 && n_local >= 0 && n_sink + n_local <= n_blocks,
+              "n_blocks must be positive and hold n_sink + n_local blocks");
+  const c10::cuda::CUDAGuard guard(score.device());
+  auto out = torch::empty({rows, n_blocks}, score.options().dtype(at::kInt));
+  check_status(hcu_select_blocks(ptr<const float>(score), rows, score.size(1), score.stride(0),
+                                 ptr<const int16_t>(nonzero_mask), nonzero_mask.stride(0), ptr<const int32_t>(lengths),
+                                 n_blocks, n_sink, n_local, ptr<int32_t>(out), cur_stream()),
+               "select_blocks");
+  return out;
+}
+
+// [slots, 1, width] / [slots, width] uint8 cache: (slots, slot stride).
+std::pair<int64_t, int64_t> slot_rows(const torch::Tensor& kv, int64_t width) {
+  TORCH_CHECK(kv.is_cuda() && kv.element_size() == 1 && kv.dim() >= 2 && kv.size(-1) == width && kv.stride(-1) == 1 &&
+                  kv.numel() == kv.size(0) * width && (kv.size(0) <= 1 || kv.stride(0) >= width) &&
+                  kv.stride(0) % 16 == 0,
+              "the cache must be bytes [slots, 1, ", width, "] with unit last stride and 16-byte aligned slots");
+  return {kv.size(0), std::max(kv.stride(0), width)};
+}
+
+torch::Tensor store_mla_kv4(const torch::Tensor& kv_c, const torch::Tensor& k_pe, const torch::Tensor& loc,
+                            torch::Tensor kv_buffer) {
+  const auto [slots, stride] = slot_rows(kv_buffer, 432);
+  TORCH_CHECK(kv_c.scalar_type() == at::kBFloat16 && k_pe.scalar_type() == at::kBFloat16,
+              "kv_c and k_pe must be bfloat16");
+  const int64_t ks = row_stride(kv_c, 512), ps = row_stride(k_pe, 64);
+  TORCH_CHECK(loc.scalar_type() == at::kLong && loc.dim() == 1 && loc.is_contiguous() &&
+                  loc.size(0) <= kv_c.size(0) && kv_c.size(0) == k_pe.size(0),
+              "loc must be contiguous int64 [n], n at most the tokens of kv_c and k_pe");
+  TORCH_CHECK(kv_c.device() == kv_buffer.device() && k_pe.device() == kv_buffer.device() &&
+                  loc.device() == kv_buffer.device(),
+              "all tensors must be on the cache's device");
+  TORCH_CHECK(ks % 8 == 0 && reinterpret_cast<uintptr_t>(kv_c.data_ptr()) % 16 == 0,
+              "kv_c rows must be 16-byte aligned");
+  const c10::cuda::CUDAGuard guard(kv_buffer.device());
+  check_status(hcu_store_mla_kv4(ptr<const uint16_t>(kv_c), ks, ptr<const uint16_t>(k_pe), ps, ptr<const int64_t>(loc),
+                                 loc.size(0), ptr<uint8_t>(kv_buffer), slots, stride, cur_stream()),
+               "store_mla_kv4");
+  return kv_buffer;
+}
+
+torch::Tensor dequantize_mla_kv4_paged(const torch::Tensor& kv_buffer, const torch::Tensor& page_table_1) {
+  const auto [slots, stride] = slot_rows(kv_buffer, 432);
+  TORCH_CHECK(page_table_1.scalar_type() == at::kInt && page_table_1.dim() == 1 && page_table_1.is_contiguous() &&
+                  page_table_1.device() == kv_buffer.device(),
+              "page_table_1_flattened must be contiguous int32 [n] on the cache's device");
+  const c10::cuda::CUDAGuard guard(kv_buffer.device());
+  const int64_t n = page_table_1.size(0);
+  auto out = torch::empty({n, 1, 576}, kv_buffer.options().dtype(at::kBFloat16));
+  check_status(hcu_dequant_mla_kv4_paged(ptr<const uint8_t>(kv_buffer), slots, stride, ptr<const int32_t>(page_table_1),
+                                         n, ptr<uint16_t>(out), cur_stream()),
+               "dequantize_mla_kv4_paged");
+  return out;
+}
+
+std::vector<torch::Tensor> sparse_mla_attention(const torch::Tensor& q, const torch::Tensor& kv_cache,
+                                                const torch::Tensor& indices,
+                                                const c10::optional<torch::Tensor>& block_table,
+                                                const c10::optional<torch::Tensor>& lengths, double sm_scale) {
+  TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.size(2) == 576 &&
+                  q.size(1) >= 1 && q.stride(2) == 1 && q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+              "q must be bfloat16 [rows, heads, 576] with a unit last stride and 16-byte aligned rows");
+  const bool fp4 = kv_cache.dim() >= 2 && kv_cache.size(-1) == 432;
+  const auto [slots, stride] = slot_rows(kv_cache, fp4 ? 432 : 656);
+  const int64_t R = q.size(0), H = q.size(1);
+  const auto rows2d = [&](const torch::Tensor& t) {
+    return t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) == R && (t.numel() == 0 || t.stride(1) == 1) &&
+           t.device() == q.device();
+  };
+  TORCH_CHECK(rows2d(indices), "indices must be row-contiguous int32 [rows, n] on q's device");
+  TORCH_CHECK(kv_cache.device() == q.device(), "kv_cache must be on q's device");
+  TORCH_CHECK(block_table.has_value() == lengths.has_value(), "block_table and lengths come together");
+  if (block_table.has_value()) {
+    TORCH_CHECK(rows2d(*block_table), "block_table must be row-contiguous int32 [rows, pages] on q's device");
+    TORCH_CHECK(lengths->scalar_type() == at::kInt && lengths->dim() == 1 && lengths->is_contiguous() &&
+                    lengths->size(0) == R && lengths->device() == q.device(),
+                "lengths must be contiguous int32 [rows] on q's device");
+  }
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto out = torch::empty({R, H, 512}, q.options());
+  auto lse = torch::empty({R, H}, q.options().dtype(at::kFloat));
+  const int64_t n = indices.size(1);
+  const int64_t wsb = hcu_sparse_mla_attention_workspace_bytes(R, H, block_table.has_value() ? 64 * n : n);
+  TORCH_CHECK(wsb >= 0, "sparse_mla_attention: bad shape");
+  auto ws = torch::empty({wsb}, q.options().dtype(at::kByte));
+  check_status(
+      hcu_sparse_mla_attention(ptr<const uint16_t>(q), R, H, q.stride(0), q.stride(1), ptr<const uint8_t>(kv_cache),
+                               slots, stride, fp4 ? HCU_KV_FP4_432 : HCU_KV_FP8_656, ptr<const int32_t>(indices), n,
+                               indices.stride(0), block_table.has_value() ? ptr<const int32_t>(*block_table) : nullptr,
+                               block_table.has_value() ? block_table->stride(0) : 0,
+                               block_table.has_value() ? block_table->size(1) : 0,
+                               lengths.has_value() ? ptr<const int32_t>(*lengths) : nullptr,
+                               static_cast<float>(sm_scale), ws.data_ptr(), wsb, ptr<uint16_t>(out), ptr<float>(lse),
+                               cur_stream()),
+      "sparse_mla_attention");
+  return {out, lse};
+}
+
 void set_wait_limit_ns(int64_t ns) {
   TORCH_CHECK(ns >= 0, "the wait limit must be >= 0 (0: the default)");
   check_status(hcu_set_wait_limit_ns(static_cast<uint64_t>(ns)), "set_wait_limit_ns");
@@ -612,5 +763,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cp_peer_finish", &cp_peer_finish, "context-parallel over peer memory: wait for every rank's rows");
   m.def("topk_keys_if", &topk_keys_if, "topk_keys predicated on a device word (does nothing when it is 0)");
   m.def("set_wait_limit_ns", &set_wait_limit_ns, "limit of the library's bounded waits (0: default 2 s)");
+  m.def("step_tables", &step_tables, "block tables, slot maps and page allocation of one step");
+  m.def("select_blocks", &select_blocks, "top-n 64-token blocks of each row by the indexer's scores");
+  m.def("store_mla_kv4", &store_mla_kv4, "4-bit MLA slot writer");
+  m.def("dequantize_mla_kv4_paged", &dequantize_mla_kv4_paged, "4-bit MLA slot dequant -> bf16 [n, 1, 576]");
+  m.def("sparse_mla_attention", &sparse_mla_attention,
+        "MLA attention over selected tokens (slots) or blocks (block table and lengths)");
   m.def("version", []() { return std::string(hcu_version()); });
 }

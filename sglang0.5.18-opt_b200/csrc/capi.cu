@@ -57,6 +57,10 @@ extern "C" int hcu_read_device_status(uint32_t* status, int clear) {
   if (e == cudaSuccess) e = hcu::status_topk(status, clear);
   if (e == cudaSuccess) e = hcu::status_logits(status, clear);
   if (e == cudaSuccess) e = hcu::status_mla(status, clear);
+  if (e == cudaSuccess) e = hcu::status_tables(status, clear);
+  if (e == cudaSuccess) e = hcu::status_blocks(status, clear);
+  if (e == cudaSuccess) e = hcu::status_kv4(status, clear);
+  if (e == cudaSuccess) e = hcu::status_sparse_mla(status, clear);
   if (e != cudaSuccess) {
     hcu::set_last_error(e);
     return HCU_ERR_LAUNCH;
@@ -70,6 +74,7 @@ extern "C" int hcu_set_wait_limit_ns(uint64_t ns) {
   if (e == cudaSuccess) e = hcu::status_topk_set_wait_limit(ns);
   if (e == cudaSuccess) e = hcu::status_logits_set_wait_limit(ns);
   if (e == cudaSuccess) e = hcu::status_mla_set_wait_limit(ns);
+  if (e == cudaSuccess) e = hcu::status_sparse_mla_set_wait_limit(ns);
   if (e != cudaSuccess) {
     hcu::set_last_error(e);
     return HCU_ERR_LAUNCH;

@@ -428,8 +428,13 @@ cudaError_t status_dequant(uint32_t* out, int clear);
 cudaError_t status_topk(uint32_t* out, int clear);
 cudaError_t status_logits(uint32_t* out, int clear);
 cudaError_t status_mla(uint32_t* out, int clear);
+cudaError_t status_tables(uint32_t* out, int clear);
+cudaError_t status_blocks(uint32_t* out, int clear);
+cudaError_t status_kv4(uint32_t* out, int clear);
+cudaError_t status_sparse_mla(uint32_t* out, int clear);
 cudaError_t status_dequant_set_wait_limit(uint64_t ns);
 cudaError_t status_topk_set_wait_limit(uint64_t ns);
 cudaError_t status_logits_set_wait_limit(uint64_t ns);
 cudaError_t status_mla_set_wait_limit(uint64_t ns);
+cudaError_t status_sparse_mla_set_wait_limit(uint64_t ns);
 }  // namespace hcu

@@ -1,0 +1,271 @@
+// The 64-token blocks a row attends to, chosen by the indexer's scores.
+//
+//   m_b = max over the visible tokens of block b of (mask bit set ? score : +0)
+// and the n blocks with the largest m_b, ties to the lower index, the first n_sink and the last
+// n_local visible blocks always among them, written in ascending order (-1 pads).
+//
+// One cluster of S CTAs per row.  Every CTA streams its share of the row's blocks (half a warp per
+// block, 16 bytes a lane, 16 blocks in flight per warp), reduces each block to one monotone integer
+// key and stores it into rank 0's shared memory; after the cluster barrier rank 0 finds the n-th
+// largest key by an 8-bit radix select over the keys in its shared memory and writes the chosen
+// blocks by one block-wide scan.  With rows enough to fill the SMs S is 1 and the select of one row
+// overlaps the streams of the others on its SM.
+//
+// Bound: the read of the scores, 4 B + 1 bit per visible token.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+HCU_DEFINE_STATUS(status_blocks)
+
+namespace cg = cooperative_groups;
+
+namespace hcu {
+namespace {
+
+constexpr int kSbThreads = 256;
+constexpr int kSbWarps = kSbThreads / 32;
+constexpr int kUnit = 16;                 // blocks per warp step: 8 loads of two blocks each
+constexpr uint32_t kForced = 0xffffffffu;  // key of a block that is always chosen
+constexpr int kMaxRowBlocks = 49152;       // keys of a row held in shared memory (192 KB)
+constexpr int kMaxSbSplits = 8;            // portable cluster size
+
+struct BlocksArgs {
+  const float* score;
+  int64_t score_stride;
+  const int16_t* mask;
+  int64_t mask_stride;
+  const int32_t* lengths;
+  int width;      // tokens
+  int n;          // blocks to choose
+  int n_sink, n_local;
+  int splits;
+  int32_t* out;  // [rows, n]
+};
+
+struct SbSmem {
+  int hist[256];
+  int warp_above[kSbWarps], warp_tie[kSbWarps];
+  int bin, above;
+};
+
+// Monotone signed image of a float: a larger score has a larger image; NaN with a clear sign is
+// above +inf.
+__device__ __forceinline__ int ordered(uint32_t b) {
+  return static_cast<int>(b) ^ (static_cast<int>(static_cast<int>(b) >> 31) & 0x7fffffff);
+}
+
+__global__ __launch_bounds__(kSbThreads) void select_blocks_kernel(const BlocksArgs a) {
+  extern __shared__ uint32_t keys[];  // rank 0: one key per visible block of the row
+  __shared__ SbSmem sm;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = a.splits > 1 ? static_cast<int>(blockIdx.x) % a.splits : 0;
+  const int64_t row = a.splits > 1 ? blockIdx.x / a.splits : blockIdx.x;
+  const int len = max(0, min(__ldg(a.lengths + row), a.width));
+  const int nb = (len + kPage - 1) / kPage;
+  int32_t* out = a.out + row * a.n;
+  uint32_t* dst_keys = keys;
+  if (a.splits > 1) {
+    cg::this_cluster().sync();  // rank 0 has started: its shared memory may be written
+    dst_keys = cg::this_cluster().map_shared_rank(keys, 0);
+  }
+
+  const bool all = nb <= a.n;  // uniform over the cluster
+  if (!all) {
+    const float* score = a.score + row * a.score_stride;
+    const int16_t* mask = a.mask + row * a.mask_stride;
+    const int units = (nb + kUnit - 1) / kUnit;
+    for (int u = rank * kSbWarps + warp; u < units; u += a.splits * kSbWarps) {
+      float4 x[8];
+      uint32_t m[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // load i: blocks 2i (lanes 0-15) and 2i + 1
+        const int tok = (u * kUnit + 2 * i) * kPage + 4 * lane;
+        const bool on = tok < len;
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        m[i] = 0;
+        if (tok + 3 < len) {
+          x[i] = __ldcs(reinterpret_cast<const float4*>(score + tok));
+        } else if (on) {
+          x[i].x = score[tok];
+          if (tok + 1 < len) x[i].y = score[tok + 1];
+          if (tok + 2 < len) x[i].z = score[tok + 2];
+        }
+        if (on) m[i] = static_cast<uint32_t>(static_cast<uint16_t>(__ldg(mask + (tok >> 4)))) >> (tok & 15);
+      }
+      int k[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int tok = (u * kUnit + 2 * i) * kPage + 4 * lane;
+        // a visible token without its mask bit counts as +0 (image 0); one past the length not at all
+        const int lo = static_cast<int>(0x80000000u);
+        const int k0 = (m[i] & 1) ? ordered(__float_as_uint(x[i].x)) : 0;
+        const int k1 = (m[i] & 2) ? ordered(__float_as_uint(x[i].y)) : 0;
+        const int k2 = (m[i] & 4) ? ordered(__float_as_uint(x[i].z)) : 0;
+        const int k3 = (m[i] & 8) ? ordered(__float_as_uint(x[i].w)) : 0;
+        k[i] = tok < len ? k0 : lo;
+        if (tok + 1 < len) k[i] = max(k[i], k1);
+        if (tok + 2 < len) k[i] = max(k[i], k2);
+        if (tok + 3 < len) k[i] = max(k[i], k3);
+      }
+      // Maxima over the 16 lanes of each half warp, all eight loads at once: each step halves the
+      // loads a lane carries, so 8 values take 4 + 2 + 1 + 1 shuffles instead of 8 x 4.
+#pragma unroll
+      for (int s = 0; s < 3; ++s) {
+        const int half = 4 >> s, o = 1 << s;
+        const bool hi = lane & o;
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+          const int send = hi ? k[i] : k[i + half];
+          const int keep = hi ? k[i + half] : k[i];
+          k[i] = max(keep, __shfl_xor_sync(0xffffffffu, send, o));
+        }
+      }
+      k[0] = max(k[0], __shfl_xor_sync(0xffffffffu, k[0], 8));
+      // lane bits 0..2 name the load: bit 0 chose the upper four, bit 1 the upper two, bit 2 the last
+      const int load = ((lane & 1) << 2) | (lane & 2) | ((lane >> 2) & 1);
+      const int b = u * kUnit + 2 * load + (lane >> 4);
+      if (!(lane & 8) && b < nb) {
+        const bool forced = b < a.n_sink || b >= nb - a.n_local;
+        const int im = k[0] == -1 ? 0 : k[0];  // -0 ties with +0
+        dst_keys[b] = forced ? kForced : static_cast<uint32_t>(im) ^ 0x80000000u;
+      }
+    }
+  }
+  if (a.splits > 1)
+    cg::this_cluster().sync();  // rank 0 reads below what every rank stored above; no rank touches
+                                // another's shared memory after this barrier
+  else
+    __syncthreads();
+  if (rank != 0) return;
+  if (all) {
+    for (int i = tid; i < a.n; i += kSbThreads) out[i] = i < nb ? i : -1;
+    return;
+  }
+
+  // n-th largest key: four 8-bit digits from the top
+  uint32_t prefix = 0;
+  int left = a.n;  // rank of the wanted key among the keys that match the prefix
+#pragma unroll
+  for (int d = 24; d >= 0; d -= 8) {
+    sm.hist[tid] = 0;
+    __syncthreads();
+    const uint32_t hi_mask = d == 24 ? 0u : 0xffffffffu << (d + 8);
+    for (int b = tid; b < nb; b += kSbThreads) {
+      const uint32_t k = keys[b];
+      if ((k & hi_mask) == prefix) atomicAdd(&sm.hist[(k >> d) & 255], 1);
+    }
+    __syncthreads();
+    if (warp == 0) {  // lane l: bins 8l .. 8l + 7; suffix sums over lanes from the top
+      int c[8], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += c[j] = sm.hist[8 * lane + j];
+      int suf = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_down_sync(0xffffffffu, suf, o);
+        if (lane + o < 32) suf += y;
+      }
+      int above = suf - sum;  // keys in higher lanes' bins
+      if (above < left && suf >= left) {
+#pragma unroll
+        for (int j = 7; j >= 0; --j) {
+          if (above < left && above + c[j] >= left) {
+            sm.bin = 8 * lane + j;
+            sm.above = above;
+          }
+          above += c[j];
+        }
+      }
+    }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(sm.bin) << d;
+    left -= sm.above;
+    __syncthreads();
+  }
+
+  // prefix: the threshold key; `left` of the keys equal to it are taken, lowest blocks first
+  const int per = (nb + kSbThreads - 1) / kSbThreads;
+  const int b0 = min(tid * per, nb), b1 = min(b0 + per, nb);
+  int above = 0, tie = 0;
+  for (int b = b0; b < b1; ++b) {
+    above += keys[b] > prefix;
+    tie += keys[b] == prefix;
+  }
+  int ia = above, it = tie;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int ya = __shfl_up_sync(0xffffffffu, ia, o), yt = __shfl_up_sync(0xffffffffu, it, o);
+    if (lane >= o) {
+      ia += ya;
+      it += yt;
+    }
+  }
+  if (lane == 31) {
+    sm.warp_above[warp] = ia;
+    sm.warp_tie[warp] = it;
+  }
+  __syncthreads();
+  int na = ia - above, nt = it - tie;
+  for (int w = 0; w < warp; ++w) {
+    na += sm.warp_above[w];
+    nt += sm.warp_tie[w];
+  }
+  for (int b = b0; b < b1; ++b) {
+    const uint32_t k = keys[b];
+    if (k > prefix) {
+      out[na + min(nt, left)] = b;
+      ++na;
+    } else if (k == prefix) {
+      if (nt < left) out[na + nt] = b;
+      ++nt;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace hcu
+
+extern "C" int hcu_select_blocks(const float* score, int64_t rows, int64_t width, int64_t score_stride,
+                                 const int16_t* mask, int64_t mask_stride, const int32_t* lengths, int64_t n_blocks,
+                                 int64_t n_sink, int64_t n_local, int32_t* out, hcu_stream_t stream) {
+  using namespace hcu;
+  if (rows < 0 || width < 0 || score_stride < width || score_stride % 4 != 0 || mask_stride < (width + 15) / 16 ||
+      n_blocks < 1 || n_sink < 0 || n_local < 0 || n_sink + n_local > n_blocks)
+    return HCU_ERR_ARG;
+  if (rows == 0) return HCU_OK;
+  const int64_t row_blocks = (width + kPage - 1) / kPage;
+  if (row_blocks > kMaxRowBlocks || n_blocks > 0x7fffffff || rows > 0x7fffffff / kMaxSbSplits)
+    return HCU_ERR_UNSUPPORTED;
+  if (!lengths || !out || (width > 0 && (!score || !mask))) return HCU_ERR_ARG;
+  if (reinterpret_cast<uintptr_t>(score) % 16 != 0) return HCU_ERR_ARG;
+  BlocksArgs a{score, score_stride, mask, mask_stride, lengths, static_cast<int>(width), static_cast<int>(n_blocks),
+               static_cast<int>(n_sink), static_cast<int>(n_local), 1, out};
+  // Splits: enough CTAs to give every SM about two, each with 64 blocks (4096 tokens) at least.
+  int s = 1;
+  while (s < kMaxSbSplits && rows * 2 * s <= 2 * sm_count() && row_blocks >= 2 * s * 64) s *= 2;
+  a.splits = s;
+  const size_t smem = static_cast<size_t>(row_blocks) * sizeof(uint32_t);
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(select_blocks_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kMaxRowBlocks * static_cast<int>(sizeof(uint32_t)));
+    if (e != cudaSuccess) {
+      set_last_error(e);
+      return HCU_ERR_LAUNCH;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * s));
+  cfg.blockDim = dim3(kSbThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(s);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = s > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, select_blocks_kernel, a);
+  return launch_status();
+}

@@ -14,6 +14,7 @@ behind ``_C``.  There is no fallback: importing this package fails if the
 extension has not been built (``python build.py`` next to this package).
 """
 import os
+from typing import NamedTuple
 
 import torch  # noqa: F401  (loads libtorch before the extension)
 
@@ -278,6 +279,72 @@ def rope_qout_kv_store(positions, q_pe, q_out, kv_c, kv_weight, norm_eps, k_pe, 
     128-element groups, 4 fp32 scales, the rotated k_pe as bf16)."""
     _C.rope_qout_kv_store(positions.reshape(-1), q_pe, q_out, kv_c, kv_weight, float(norm_eps), k_pe,
                           cos_sin_cache, bool(is_neox), kv_buffer, loc, float(store_eps), _RSQRT_MODE)
+
+
+# --- sparse attention around the indexer ------------------------------------------------------------
+class StepTables(NamedTuple):
+    """What ``step_tables`` returns; the shapes are those the other ops of a step take."""
+    block_table: torch.Tensor        # int32 [rows, width / 64], -1 after the request's pages
+    page_table_size_1: torch.Tensor  # int32 [rows, width], -1 after the request's tokens
+    lengths: torch.Tensor            # int32 [rows]: visible tokens (context_lens of mqa_logits, lengths of the top-k)
+    positions: torch.Tensor          # int32 [rows]
+    token_loc: torch.Tensor          # int32 [rows]: the new token's slot (quant_store_index_k)
+    loc: torch.Tensor                # int64 [rows]: the same (rope_qout_kv_store, store_mla_kv4)
+    free_head: torch.Tensor          # int32 [1]: the next step's free_head
+
+
+def step_tables(req_pages, req_idx, seq_lens, new_lens, free_pages, free_head, n_rows, width):
+    """Block tables, slot maps and lengths of one decode or prefill step, built on the GPU in one launch.
+
+    Request ``i`` of the step is row ``req_idx[i]`` of ``req_pages`` (int32 ``[requests, max_pages]``, page ids
+    of 64 tokens), has ``seq_lens[i]`` cached tokens and brings ``new_lens[i]`` new ones (all int32).  The pages
+    that the new tokens need come from ``free_pages`` in order, from ``free_head[0]`` on, and are written into
+    ``req_pages`` in place.  The query rows are the new tokens, request by request; ``n_rows`` may exceed their
+    number (a padded batch): the rows after them are empty (length 0, entries -1).  ``width`` (a multiple of 64)
+    is the tokens per row of the tables.  Nothing is read on the host, so a step can be captured in a CUDA graph;
+    pages that run out, requests that outgrow the tables and bad lengths give -1 entries and set the device
+    status bit 2 (``read_device_status``)."""
+    return StepTables(*_C.step_tables(req_pages, req_idx, seq_lens, new_lens, free_pages, free_head, int(n_rows),
+                                      int(width)))
+
+
+def select_blocks(score, nonzero_mask, lengths, n_blocks, n_sink=1, n_local=1):
+    """The ``n_blocks`` 64-token blocks of each row with the largest indexer scores, ascending, -1 pads
+    (int32 ``[rows, n_blocks]``).
+
+    ``score`` / ``nonzero_mask`` / ``lengths`` as ``mqa_logits`` (or ``mqa_logits_ragged``) and the top-k take
+    them: a block's score is the largest of its visible tokens', a token without its mask bit counting as +0;
+    ties go to the lower block.  The first ``n_sink`` and the last ``n_local`` visible blocks are always chosen."""
+    return _C.select_blocks(score, nonzero_mask, lengths, int(n_blocks), int(n_sink), int(n_local))
+
+
+def sparse_mla_attention(q, kv_cache, indices, sm_scale):
+    """MLA attention of ``q`` (bf16 ``[rows, heads, 576]``, the absorbed query and its rope) over the slots
+    ``indices`` (int32 ``[rows, n]``, negative entries skipped: what ``sparse_mask_topk_transform`` returns).
+
+    ``kv_cache``: uint8 ``[slots, 1, 656]`` (``rope_qout_kv_store``) or ``[slots, 1, 432]``
+    (``store_mla_kv4``).  Returns ``(out, lse)``: bf16 ``[rows, heads, 512]`` = softmax(sm_scale q k) k[:512] and
+    float32 ``[rows, heads]`` = log sum exp; a row without tokens gives 0 and -inf."""
+    return tuple(_C.sparse_mla_attention(q, kv_cache, indices, None, None, float(sm_scale)))
+
+
+def block_sparse_mla_attention(q, kv_cache, block_idx, block_table, lengths, sm_scale):
+    """``sparse_mla_attention`` over whole 64-token blocks: ``block_idx`` int32 ``[rows, n]`` names blocks of the
+    row (``select_blocks``, negative entries skipped), block ``b`` is page ``block_table[row, b]`` and its tokens at
+    positions below ``lengths[row]`` count."""
+    return tuple(_C.sparse_mla_attention(q, kv_cache, block_idx, block_table, lengths, float(sm_scale)))
+
+
+def store_mla_kv4(kv_c, k_pe, loc, kv_buffer):
+    """Writes normed latents ``kv_c`` (bf16 ``[T, 512]``, finite) and rotated ropes ``k_pe`` (bf16 ``[T, 64]``) into
+    the 432-byte 4-bit slots ``kv_buffer[loc]`` (uint8 ``[slots, 1, 432]``) in place: e2m1 codes with an e4m3
+    scale per 16 elements and a power-of-two scale per token, the rope in bf16.  ``loc``: int64 ``[n <= T]``."""
+    return _C.store_mla_kv4(kv_c, k_pe, loc, kv_buffer)
+
+
+def dequantize_mla_kv4_paged(kv_buffer, page_table_1_flattened):
+    """``dequantize_k_cache_paged`` for 432-byte slots -> bf16 ``[n, 1, 576]`` (the exact values)."""
+    return _C.dequantize_mla_kv4_paged(kv_buffer, page_table_1_flattened)
 
 
 def read_device_status(clear=True):
