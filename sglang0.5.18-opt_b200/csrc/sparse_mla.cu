@@ -12,10 +12,11 @@
 //   * 8 loader warps (one 8-token swizzle group each) gather the slots with 16-byte loads into
 //     registers, convert them to f16 and store them as the tile's K: 9 chunks of [64 tokens][64
 //     values], rows of 128 bytes, 128-byte swizzle.  A chunk is a K-major operand for q k^T and, read
-//     the other way, an MN-major one for v^T, so the latent is stored once.  Raw loads of the next
-//     tile are issued as the registers of this one are consumed;
-//   * the MMA thread issues S = Q K^T (M = 64 heads, N = 64 tokens, K = 576) and, one tile behind,
-//     O^T += V^T P^T (M = 128 latent values x 4, N = heads, K = 64 tokens): with the latent as M both
+//     the other way, an MN-major one for v^T, so the latent is stored once.  The next tile's loads go
+//     out as soon as this one is stored;
+//   * 3 warps convert each segment's Q (f16, K-major);
+//   * the MMA thread issues S = Q K^T (M = 64 heads, N = 64 tokens, K = 576) and, up to two tiles
+//     behind, O^T += V^T P^T (M = 128 latent values x 4, N = heads, K = 64 tokens): with the latent as M both
 //     products run without padding rows at 64 heads, and O^T takes 4 x 64 TMEM columns;
 //   * 4 softmax warps (16 heads each) read S, keep the running maximum and sum in fp32 and write P
 //     in f16 over the tile's rope chunk, which S no longer needs.  O^T is rescaled only when a
@@ -34,7 +35,11 @@
 // Bound: at 64 heads the shared-memory port.  A 64-token tile moves 72 KB of K in, 147 KB of Q and K
 // operands for S and 96 KB of V and P for O out: about 2500 cycles at 128 B per cycle, 39 per token,
 // against 24 per token for its products at the dense rate and 15 for its share of HBM.
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
+
+#include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "mla_slots.cuh"
@@ -44,19 +49,24 @@ HCU_DEFINE_STATUS(status_sparse_mla)
 namespace hcu {
 namespace {
 
-constexpr int kTile = 64;        // candidates per tile
+constexpr int kTile = 48;        // candidates per tile
 constexpr int kHg = 64;          // heads per job
 constexpr int kChunks = kQkDim / 64;
-constexpr int kChunkBytes = 64 * 128;  // [64 rows][64 f16]
-constexpr int kTileBytes = kChunks * kChunkBytes;
+constexpr int kQChunk = kHg * 128;     // [64 heads][64 f16]
+constexpr int kChunk = kTile * 128;    // [48 tokens][64 f16]
+constexpr int kTileBytes = kChunks * kChunk;
+constexpr int kRawFp8 = 704, kRawFp4 = 480;  // a slot's row in the raw buffer (see Raw), the slot padded with zeros
 constexpr int kSoftWarps = 4;
 constexpr int kMmaWarp = kSoftWarps;
-constexpr int kLoadWarp = kSoftWarps + 1;
-constexpr int kLoadWarps = 8;
+constexpr int kGatherWarp = kMmaWarp + 1;
+constexpr int kQWarp = kGatherWarp + 1;
+constexpr int kQWarps = 3;
+constexpr int kLoadWarp = kQWarp + kQWarps;
+constexpr int kLoadWarps = kTile / 8;
 constexpr int kAtThreads = (kLoadWarp + kLoadWarps) * 32;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kTmemO = 0;    // 4 blocks of 128 latent values x 64 heads
-constexpr uint32_t kTmemS = 256;  // 2 score buffers of 64 columns
+constexpr uint32_t kTmemS = 256;  // 2 score buffers of 48 columns, 64 apart
 // P is 2^(w - m + kBias): a row's largest weight is 2^11, 2^15 while its maximum has grown by the
 // tolerated 2^kLazy, and weights down to 2^-25 of the largest are normal f16 numbers.
 constexpr float kLazy = 4.f;
@@ -65,16 +75,19 @@ constexpr int kRopeShift = 10;
 constexpr int kPartFloats = kHg * kLatentDim + kHg;
 
 struct __align__(1024) AtSmem {
-  uint8_t q[kTileBytes];
+  uint8_t q[kChunks * kQChunk];
   uint8_t k[2][kTileBytes];
+  __align__(128) uint8_t raw[kTile * kRawFp8];  // slots of the tile to be converted next, as they are in the cache
+  __align__(16) uint8_t stage[kSoftWarps][1024];  // output rows on their way out
   float tok_e[2][kTile];    // E of each token (-inf: no token)
   float tok_up[2][kTile];   // 2^E (0: no token)
   float tok_dn[2][kTile];   // 2^-E (0: no token)
-  float cq[2][kHg];         // per head: 2^e * sm_scale * log2(e), beside a segment's first tile
+  float cq[4][kHg];         // per segment and head: 2^e * sm_scale * log2(e)
   float factor[kHg];        // rescale of O, then 1 / sum
-  int empty_tile[2];        // the tile holds no token
+  uint32_t mask[2];         // candidates in raw that are tokens
+  int empty_tile[2];        // the tile in buffer b holds no token
   uint64_t full[2], empty[2], sfull[2], pready[2];
-  uint64_t qfull, qempty, oempty, done;
+  uint64_t rfull, rempty, qfull, qempty, oempty, done;
   uint32_t tmem;
   int abort;
 };
@@ -125,25 +138,48 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool a_mn) {
 __device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-  d |= static_cast<uint64_t>(kChunkBytes >> 4) << 16;  // leading offset: next 64 M values
+  d |= static_cast<uint64_t>(kChunk >> 4) << 16;  // leading offset: next 64 M values
   d |= static_cast<uint64_t>(1024 >> 4) << 32;         // stride offset: next 8 K rows
   d |= static_cast<uint64_t>(1) << 46;
   d |= static_cast<uint64_t>(2) << 61;
   return d;
 }
 
-// 16 lanes x 64 columns, as 8 column groups of an 8x8-pair fragment: thread t holds, for group n,
-// rows t / 4 (r[4n], r[4n + 1]) and t / 4 + 8 (r[4n + 2], r[4n + 3]), columns 8n + 2 (t % 4) + {0, 1}.
-__device__ __forceinline__ void tmem_ld_16x256_x8(uint32_t taddr, uint32_t (&r)[32]) {
+// K-major operand in rows of 32 bytes (16 K values) with the 32-byte swizzle, 8 rows per 256 bytes.
+__device__ __forceinline__ uint64_t sw32_kmajor_desc(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(1) << 16;          // leading offset (unused: one 32-byte row of K)
+  d |= static_cast<uint64_t>(256 >> 4) << 32;   // stride offset: next 8 rows
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(6) << 61;
+  return d;
+}
+
+// 16 lanes x 48 columns, as 6 column groups of an 8x8-pair fragment: thread t holds, for group n, rows
+// t / 4 (r[4n], r[4n + 1]) and t / 4 + 8 (r[4n + 2], r[4n + 3]), columns 8n + 2 (t % 4) + {0, 1}.
+__device__ __forceinline__ void tmem_ld_scores(uint32_t taddr, uint32_t (&r)[24]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%24];\n\t"
+      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%25];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
         "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
-        "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
-        "=r"(r[30]), "=r"(r[31])
+        "=r"(r[23])
+      : "r"(taddr), "r"(taddr + 32)
+      : "memory");
+}
+
+// The same of 32 columns.
+__device__ __forceinline__ void tmem_ld_16x256_x4(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
 }
@@ -165,8 +201,42 @@ __device__ __forceinline__ void stmatrix_x4(uint32_t addr, uint32_t a, uint32_t 
                : "memory");
 }
 
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b),
+               "r"(c), "r"(d)
+               : "memory");
+}
+
+// 16-byte piece `part` of row h in rows of 32 bytes with the 32-byte swizzle: the pieces of every
+// other group of four rows swapped, so that eight rows' pieces fall into different banks.
+__device__ __forceinline__ int st_piece(int h, int part) { return h * 32 + ((part ^ ((h >> 2) & 1)) << 4); }
+
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+template <int kOffset = 0>
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+  asm volatile("st.shared.v4.b32 [%0 + %5], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d), "n"(kOffset)
+               : "memory");
+}
+
+// f(0), .., f(7) with the index as a constant.
+template <typename F>
+__device__ __forceinline__ void unroll8(F&& f) {
+  f(std::integral_constant<int, 0>());
+  f(std::integral_constant<int, 1>());
+  f(std::integral_constant<int, 2>());
+  f(std::integral_constant<int, 3>());
+  f(std::integral_constant<int, 4>());
+  f(std::integral_constant<int, 5>());
+  f(std::integral_constant<int, 6>());
+  f(std::integral_constant<int, 7>());
 }
 
 __device__ __forceinline__ void fence_async_shared() {
@@ -177,6 +247,19 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Whether the phase of the given parity has completed (no wait).
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, P;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 // OR of a predicate over the softmax warps.
@@ -195,105 +278,141 @@ __device__ __forceinline__ bool soft_any(bool p) {
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-__device__ __forceinline__ uint4 ldg_v4(const uint8_t* p) {
+__device__ __forceinline__ uint4 ldg_v4(const void* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
 }
+__device__ __forceinline__ uint2 ld_shared_v2(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ldg_u32(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+// Asynchronous copy of four slots (rows of the map, one row per box) into consecutive rows of shared
+// memory; a row out of range (-1) and the box's bytes past the slot are filled with zeros.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int r0, int r1, int r2,
+                                            int r3) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
+      : "memory");
+}
 
-// ---------------------------------------------------------------- loader
-// One lane's view of a tile's candidates.
-struct Cand {
-  int32_t a, b;  // token form: slots of candidates 2 lane, 2 lane + 1 (-1: none); block form: first slot, count
-  bool any;      // the tile holds a token (uniform)
+// ---------------------------------------------------------------- gather
+// Lane l < 12 of the gather warp looks up candidates 4 l .. 4 l + 3 of each tile, in stages a tile apart
+// so that no load waits for the one that names it: list entries, then (block form) the page and the
+// row's length.  What a stage loads is not touched before the next one (a select on it would wait for
+// it): places past the list's end or the CTA's range read some entry of it and are marked instead.
+constexpr int kGatherLanes = kTile / 4;
+struct Entry {
+  int32_t v[4];  // list entries: slots, or blocks
+  int in;        // bit i: v[i] lies in the list
+};
+struct Place {
+  int32_t v[4];    // token form: slots; block form: pages
+  int32_t len;     // block form: the row's length
+  int32_t pos[4];  // block form: the candidates' positions in the row
+  int in;          // bit i: a candidate; bit 4 + i: its block lies past the table
 };
 
 template <bool kBlocks>
-__device__ __forceinline__ Cand candidates(const AttnArgs& p, int64_t row, int tile, int lane) {
-  Cand c;
-  if constexpr (kBlocks) {
-    c.a = c.b = 0;
-    const int32_t b = tile < p.n_idx ? __ldg(p.idx + row * p.idx_stride + tile) : -1;
-    if (b >= 0) {
-      const int64_t left = static_cast<int64_t>(__ldg(p.lengths + row)) - static_cast<int64_t>(b) * kPage;
-      const int n = left <= 0 ? 0 : static_cast<int>(left < kPage ? left : kPage);
-      const int32_t page = n > 0 && b < p.n_bt ? __ldg(p.bt + row * p.bt_stride + b) : -1;
-      const int64_t s = static_cast<int64_t>(page) * kPage;
-      if (page >= 0 && s + n <= p.n_slots) {
-        c.a = static_cast<int32_t>(s);
-        c.b = n;
-      } else if (n > 0 && lane == 0) {
-        atomicOr(&g_hcu_status, HCU_STATUS_BAD_INPUT);
-      }
+__device__ __forceinline__ Entry load_entry(const AttnArgs& p, int64_t row, int tile, int lane, bool on) {
+  Entry e;
+  const int32_t* p0 = p.idx + (on ? row : 0) * p.idx_stride;
+  const int last = on && lane < kGatherLanes ? p.n_idx - 1 : -1;
+  e.in = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    int j = tile * kTile + 4 * lane + i;
+    if constexpr (kBlocks) j /= kPage;
+    e.v[i] = static_cast<int32_t>(ldg_u32(p0 + max(min(j, last), 0)));
+    e.in |= j <= last ? 1 << i : 0;
+  }
+  return e;
+}
+
+template <bool kBlocks>
+__device__ __forceinline__ Place load_place(const AttnArgs& p, int64_t row, int tile, int lane, const Entry& e) {
+  Place c;
+  c.in = e.in;
+  c.len = kBlocks ? static_cast<int32_t>(ldg_u32(p.lengths + (e.in ? row : 0))) : 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    c.v[i] = e.v[i];
+    if constexpr (kBlocks) {
+      const bool on = (e.in >> i & 1) && e.v[i] >= 0;
+      c.pos[i] = on ? e.v[i] * kPage + (tile * kTile + 4 * lane + i) % kPage : 0;
+      c.v[i] = static_cast<int32_t>(
+          ldg_u32(p.bt + (on ? row : 0) * p.bt_stride + max(min(on ? e.v[i] : 0, p.n_bt - 1), 0)));
+      c.in = (c.in & ~(1 << i)) | (on ? 1 << i : 0) | (on && e.v[i] >= p.n_bt ? 16 << i : 0);
     }
-    c.any = c.b > 0;
-  } else {
-    const int j = tile * kTile + 2 * lane;
-    const int32_t* p0 = p.idx + row * p.idx_stride;
-    c.a = j < p.n_idx ? __ldg(p0 + j) : -1;
-    c.b = j + 1 < p.n_idx ? __ldg(p0 + j + 1) : -1;
-    const bool bad_a = c.a >= p.n_slots, bad_b = c.b >= p.n_slots;
-    if (bad_a || bad_b) atomicOr(&g_hcu_status, HCU_STATUS_BAD_INPUT);
-    if (bad_a) c.a = -1;
-    if (bad_b) c.b = -1;
-    c.any = __any_sync(0xffffffffu, c.a >= 0 || c.b >= 0);
   }
   return c;
 }
 
-// Slot of candidate j of the tile (uniform), -1 where there is none.
+// Slot of candidate i of the lane, -1: none.
 template <bool kBlocks>
-__device__ __forceinline__ int32_t slot_at(const Cand& c, int j) {
-  if constexpr (kBlocks) return j < c.b ? c.a + j : -1;
-  return __shfl_sync(0xffffffffu, j & 1 ? c.b : c.a, j >> 1);
+__device__ __forceinline__ int32_t resolve(const AttnArgs& p, const Place& c, int i) {
+  if (!(c.in >> i & 1)) return -1;
+  int64_t s = c.v[i];
+  bool bad;
+  if constexpr (kBlocks) {
+    if (c.pos[i] >= c.len) return -1;
+    s = s * kPage + c.pos[i] % kPage;
+    bad = (c.in >> (4 + i) & 1) || c.v[i] < 0 || s >= p.n_slots;
+  } else {
+    if (s < 0) return -1;
+    bad = s >= p.n_slots;
+  }
+  if (bad) atomicOr(&g_hcu_status, HCU_STATUS_BAD_INPUT);
+  return bad ? -1 : static_cast<int32_t>(s);
 }
 
-// A lane's raw bytes of its warp's 8 tokens of one tile.
+// ---------------------------------------------------------------- loader
+// Lane l of loader warp lw owns a quarter (sub = l % 4) of token 8 lw + l / 4: latent elements
+// 64 i + 16 sub .. + 15 of every chunk i and rope elements 16 sub .. + 15.  A quarter warp's two tokens
+// fall into different halves of the swizzle, so the converted 16-byte pieces store without bank
+// conflicts, all addresses are one register plus constants, and scales stay in their own lane; the raw
+// rows' strides (704 and 480 bytes) put the same lanes' raw pieces into different banks too.
 template <bool kFp4>
 struct Raw {
-  uint4 x[8];       // latent codes 16 lane .. 16 lane + 15 (4-bit: .x, .y)
-  uint32_t sc[8];   // fp8: the lane's group scale; 4-bit: its e4m3 scale
-  float ts[8];      // 4-bit: the token scale
-  uint4 rope[2];    // tokens 4 i + lane / 8, rope elements 8 (lane % 8) ..
+  uint4 x[8];   // fp8 codes
+  uint2 y[8];   // e2m1 codes
+  uint4 gs[2];  // 4-bit: the token's 32 e4m3 scales
+  uint4 sc;     // fp8: the token's 4 group scales; 4-bit: .x the token scale
+  uint4 rope[2];
 };
 
-template <bool kFp4, bool kBlocks>
-__device__ __forceinline__ void load_token(const AttnArgs& p, const Cand& c, int lw, int lane, int t, Raw<kFp4>& r) {
-  const int32_t s = slot_at<kBlocks>(c, lw * 8 + t);
-  r.x[t] = make_uint4(0, 0, 0, 0);
-  r.sc[t] = 0;
-  if constexpr (kFp4) r.ts[t] = 0.f;
-  if (s >= 0) {
-    const uint8_t* b = p.kv + s * p.slot_stride;
-    if constexpr (kFp4) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(b) + lane);
-      r.x[t].x = v.x;
-      r.x[t].y = v.y;
-      r.sc[t] = __ldg(b + kKv4Scales + lane);
-      r.ts[t] = __ldg(reinterpret_cast<const float*>(b + kKv4Token));
-    } else {
-      r.x[t] = ldg_v4(b + 16 * lane);
-      r.sc[t] = __ldg(reinterpret_cast<const uint32_t*>(b + kFp8Scales) + (lane >> 3));
-    }
+template <bool kFp4>
+__device__ __forceinline__ void read_raw(uint32_t row, int sub, Raw<kFp4>& r) {
+  if constexpr (kFp4) {
+    r.gs[0] = ld_shared_v4(row + kKv4Scales);
+    r.gs[1] = ld_shared_v4(row + kKv4Scales + 16);
+    r.sc.x = ld_shared_u32(row + kKv4Token);
+  } else {
+    r.sc = ld_shared_v4(row + kFp8Scales);
   }
-}
-
-template <bool kFp4, bool kBlocks>
-__device__ __forceinline__ void load_rope(const AttnArgs& p, const Cand& c, int lw, int lane, Raw<kFp4>& r) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int j = lw * 8 + 4 * i + (lane >> 3);
-    int32_t s;
-    if constexpr (kBlocks) {
-      s = j < c.b ? c.a + j : -1;
-    } else {
-      const int32_t a = __shfl_sync(0xffffffffu, c.a, j >> 1), b = __shfl_sync(0xffffffffu, c.b, j >> 1);
-      s = j & 1 ? b : a;
-    }
-    r.rope[i] = make_uint4(0, 0, 0, 0);
-    if (s >= 0) r.rope[i] = ldg_v4(p.kv + s * p.slot_stride + (kFp4 ? kKv4Rope : kFp8Rope) + 16 * (lane & 7));
+  for (int i = 0; i < 2; ++i) r.rope[i] = ld_shared_v4(row + (kFp4 ? kKv4Rope : kFp8Rope) + 32 * sub + 16 * i);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (kFp4)
+      r.y[i] = ld_shared_v2(row + 32 * i + 8 * sub);
+    else
+      r.x[i] = ld_shared_v4(row + 64 * i + 16 * sub);
   }
 }
 
@@ -302,118 +421,134 @@ __device__ __forceinline__ uint32_t bf2_to_h2(uint32_t w, float f) {
   return h2_bits(__floats2half2_rn(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xffff0000u) * f));
 }
 
-// The 64 heads of a job into the Q buffer: warp lw takes heads 8 lw .. 8 lw + 7, four lanes each.
-// Returns the head's factor from the product to the score in base 2.  Two passes (the second reads
-// L1) instead of 72 registers.
-__device__ __forceinline__ float load_q(const AttnArgs& p, AtSmem& sm, int64_t row, int h0, int lw, int lane) {
+// Largest magnitude among 8 packed bf16 values, per half word.
+__device__ __forceinline__ __nv_bfloat162 amax8(const uint4& v) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+  return __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3])));
+}
+// Biased exponent of the larger half of a non-negative pair (255: inf or nothing but NaN).
+__device__ __forceinline__ int exponent2(__nv_bfloat162 m) {
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(&m);
+  return static_cast<int>(max(w & 0x7fffu, w >> 16 & 0x7fffu) >> 7);
+}
+
+__device__ __forceinline__ float exp2_of(int biased) { return __uint_as_float(static_cast<uint32_t>(biased) << 23); }
+
+// Heads 8 hp .. 8 hp + 7 of a job into the Q buffer, four lanes each; cq[h] is the head's factor from
+// the product to the score in base 2.
+__device__ __forceinline__ void load_q(const AttnArgs& p, AtSmem& sm, float* cq, int64_t row, int h0, int hp,
+                                       int lane) {
   const int hr = lane >> 2, sub = lane & 3;
-  const int h = h0 + lw * 8 + hr;
-  const bool on = h < p.heads;
-  const uint4* src = reinterpret_cast<const uint4*>(p.q + row * p.q_row + static_cast<int64_t>(h) * p.q_head);
-  uint32_t am = 0;
-#pragma unroll 6
-  for (int i = 0; i < 18; ++i) {
-    const uint4 v = on ? __ldg(src + sub + 4 * i) : make_uint4(0, 0, 0, 0);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  const int h = h0 + hp * 8 + hr;
+  // a head past the last reads head 0: rows of S and columns of O are independent, and its are not stored
+  const uint4* src = reinterpret_cast<const uint4*>(p.q + row * p.q_row + (h < p.heads ? h * p.q_head : 0));
+  const uint32_t base = smem_u32(sm.q) + hp * 1024 + hr * 128;
+  uint4 v[18];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) am = max(am, max(w[j] & 0x7fffu, (w[j] >> 16) & 0x7fffu));
-  }
-  am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
-  am = max(am, __shfl_xor_sync(0xffffffffu, am, 2));
-  // biased exponent of the largest element, kept where the scales below are normal floats
-  const int eb = min(max(static_cast<int>(am >> 7), 20), 240);
-  const float f_lat = __uint_as_float(static_cast<uint32_t>(254 - eb + 3) << 23);   // largest into [2^3, 2^4)
-  const float f_rope = __uint_as_float(static_cast<uint32_t>(254 - eb + 13) << 23);  // 2^10 more
-  const uint32_t base = smem_u32(sm.q) + lw * 1024 + hr * 128;
-#pragma unroll 6
+  for (int i = 0; i < 18; ++i) v[i] = ldg_v4(src + sub + 4 * i);
+  __nv_bfloat162 am = amax8(v[0]);
+#pragma unroll
+  for (int i = 1; i < 18; ++i) am = __hmax2(am, amax8(v[i]));
+  int eb = exponent2(am);
+  eb = max(eb, __shfl_xor_sync(0xffffffffu, eb, 1));
+  eb = max(eb, __shfl_xor_sync(0xffffffffu, eb, 2));
+  eb = min(max(eb, 20), 240);  // where the factors below are normal floats
+  const float f_lat = exp2_of(254 - eb + 3);    // the largest into [2^3, 2^4)
+  const float f_rope = exp2_of(254 - eb + 13);  // 2^10 more
+#pragma unroll
   for (int i = 0; i < 18; ++i) {
     const int u = sub + 4 * i;
     const float f = i < 16 ? f_lat : f_rope;
-    const uint4 v = on ? __ldg(src + u) : make_uint4(0, 0, 0, 0);
-    st_shared_v4(base + (u >> 3) * kChunkBytes + (((u & 7) ^ hr) << 4), bf2_to_h2(v.x, f), bf2_to_h2(v.y, f),
-                 bf2_to_h2(v.z, f), bf2_to_h2(v.w, f));
+    st_shared_v4(base + (u >> 3) * kQChunk + (((u & 7) ^ hr) << 4), bf2_to_h2(v[i].x, f), bf2_to_h2(v[i].y, f),
+                 bf2_to_h2(v[i].z, f), bf2_to_h2(v[i].w, f));
   }
-  return p.sm_scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(eb - 3) << 23);
+  if (sub == 0) cq[hp * 8 + hr] = p.sm_scale * 1.4426950408889634f * exp2_of(eb - 3);
 }
 
-// Converts and stores the warp's 8 tokens of a tile; `next` (the following tile's candidates, null at
-// the end) is loaded into the registers as they fall free.
-template <bool kFp4, bool kBlocks>
-__device__ __forceinline__ void store_tile(const AttnArgs& p, AtSmem& sm, int b, const Cand& c, const Cand* next,
-                                           int lw, int lane, Raw<kFp4>& r) {
-  // rope exponents: largest biased exponent of each token's rope, at lanes 8 (t % 4) .. of er[t / 4]
-  uint32_t er[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t w[4] = {r.rope[i].x, r.rope[i].y, r.rope[i].z, r.rope[i].w};
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) m = max(m, max(w[j] & 0x7fffu, (w[j] >> 16) & 0x7fffu));
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    er[i] = m >> 7;
+// Converts the warp's 8 tokens and stores them as rows 8 lw .. 8 lw + 7 of tile buffer b; on: the
+// lane's token exists.
+template <bool kFp4>
+__device__ __forceinline__ void store_tile(AtSmem& sm, int b, int lw, int lane, bool on, const Raw<kFp4>& r) {
+  const int tok = lane >> 2, sub = lane & 3;
+  int re = exponent2(__hmax2(amax8(r.rope[0]), amax8(r.rope[1])));
+  re = max(re, __shfl_xor_sync(0xffffffffu, re, 1));
+  re = max(re, __shfl_xor_sync(0xffffffffu, re, 2));
+  uint32_t smax = r.sc.x & 0x7fffffffu;
+  if constexpr (!kFp4)
+    smax = max(max(smax, r.sc.y & 0x7fffffffu), max(r.sc.z & 0x7fffffffu, r.sc.w & 0x7fffffffu));
+  const int eb = min(max(max(static_cast<int>(smax >> 23), re - 13 - kRopeShift), 27), 247);
+  const float dn = exp2_of(254 - eb);
+  if (sub == 0) {
+    const int t = lw * 8 + tok;
+    sm.tok_e[b][t] = on ? static_cast<float>(eb - 127) : -INFINITY;
+    sm.tok_up[b][t] = on ? exp2_of(eb) : 0.f;
+    sm.tok_dn[b][t] = on ? dn : 0.f;
   }
-  uint32_t eb_rope[2] = {0, 0};
-  const uint32_t base = smem_u32(sm.k[b]) + lw * 1024;
-  const int half = (lane >> 2) & 1;  // odd chunks store their upper 16 bytes first: no bank conflict
+  // 16-byte pieces 2 sub and 2 sub + 1 of the token's row in every chunk
+  const uint32_t p0 = smem_u32(sm.k[b]) + lw * 1024 + tok * 128 + (((2 * sub) ^ tok) << 4), p1 = p0 ^ 16u;
+  const float fr = dn * (1.f / (1 << kRopeShift));
+  st_shared_v4<8 * kChunk>(p0, bf2_to_h2(r.rope[0].x, fr), bf2_to_h2(r.rope[0].y, fr),
+                                bf2_to_h2(r.rope[0].z, fr), bf2_to_h2(r.rope[0].w, fr));
+  st_shared_v4<8 * kChunk>(p1, bf2_to_h2(r.rope[1].x, fr), bf2_to_h2(r.rope[1].y, fr),
+                                bf2_to_h2(r.rope[1].z, fr), bf2_to_h2(r.rope[1].w, fr));
+  __half2 s[8];  // scale of chunk i
+  if constexpr (kFp4) {
+    const float ts = __uint_as_float(r.sc.x) * dn;
+    const uint32_t w[8] = {r.gs[0].x, r.gs[0].y, r.gs[0].z, r.gs[0].w, r.gs[1].x, r.gs[1].y, r.gs[1].z, r.gs[1].w};
 #pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    uint32_t sexp;
-    if constexpr (kFp4) {
-      sexp = (__float_as_uint(r.ts[t]) & 0x7fffffffu) >> 23;
-    } else {
-      sexp = (r.sc[t] & 0x7fffffffu) >> 23;
-      sexp = max(sexp, __shfl_xor_sync(0xffffffffu, sexp, 8));
-      sexp = max(sexp, __shfl_xor_sync(0xffffffffu, sexp, 16));
-    }
-    const int re = static_cast<int>(__shfl_sync(0xffffffffu, er[t >> 2], 8 * (t & 3)));
-    const int eb = min(max(max(static_cast<int>(sexp), re - 13 - kRopeShift), 27), 247);
-    if ((lane >> 3) == (t & 3)) eb_rope[t >> 2] = eb;
-    const float dn = __uint_as_float(static_cast<uint32_t>(254 - eb) << 23);
+    for (int i = 0; i < 8; ++i)
+      s[i] = __float2half2_rn(e4m3_to_float(static_cast<uint8_t>(w[i] >> (8 * sub))) * ts);
+  } else {
+    const uint32_t w[4] = {r.sc.x, r.sc.y, r.sc.z, r.sc.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[2 * i] = s[2 * i + 1] = __float2half2_rn(__uint_as_float(w[i]) * dn);
+  }
+  unroll8([&](auto I) {
+    constexpr int i = decltype(I)::value;
     uint32_t y[8];
     if constexpr (kFp4) {
-      const __half2 s =
-          __float2half2_rn(e4m3_to_float(static_cast<uint8_t>(r.sc[t])) * (r.ts[t] * dn));
-      const uint32_t x0 = half ? r.x[t].y : r.x[t].x, x1 = half ? r.x[t].x : r.x[t].y;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        y[i] = h2_bits(__hmul2(e2m1x2_to_half2((x0 >> (8 * i)) & 0xff), s));
-        y[4 + i] = h2_bits(__hmul2(e2m1x2_to_half2((x1 >> (8 * i)) & 0xff), s));
+      for (int k = 0; k < 4; ++k) {
+        y[k] = h2_bits(__hmul2(e2m1x2_to_half2((r.y[i].x >> (8 * k)) & 0xff), s[i]));
+        y[4 + k] = h2_bits(__hmul2(e2m1x2_to_half2((r.y[i].y >> (8 * k)) & 0xff), s[i]));
       }
     } else {
-      const __half2 s = __float2half2_rn(__uint_as_float(r.sc[t]) * dn);
-      const uint32_t x[4] = {half ? r.x[t].z : r.x[t].x, half ? r.x[t].w : r.x[t].y, half ? r.x[t].x : r.x[t].z,
-                             half ? r.x[t].y : r.x[t].w};
+      const uint32_t x[4] = {r.x[i].x, r.x[i].y, r.x[i].z, r.x[i].w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        y[2 * i] = h2_bits(__hmul2(e4m3x2_to_half2(x[i] & 0xffffu), s));
-        y[2 * i + 1] = h2_bits(__hmul2(e4m3x2_to_half2(x[i] >> 16), s));
+      for (int k = 0; k < 4; ++k) {
+        y[2 * k] = h2_bits(__hmul2(e4m3x2_to_half2(x[k] & 0xffffu), s[i]));
+        y[2 * k + 1] = h2_bits(__hmul2(e4m3x2_to_half2(x[k] >> 16), s[i]));
       }
     }
-    const uint32_t a = base + (lane >> 2) * kChunkBytes + t * 128;
-    const int u = 2 * (lane & 3) + half;
-    st_shared_v4(a + ((u ^ t) << 4), y[0], y[1], y[2], y[3]);
-    st_shared_v4(a + (((u ^ 1) ^ t) << 4), y[4], y[5], y[6], y[7]);
-    const bool on = slot_at<kBlocks>(c, lw * 8 + t) >= 0;
-    if (lane == t) {
-      sm.tok_e[b][lw * 8 + t] = on ? static_cast<float>(eb - 127) : -INFINITY;
-      sm.tok_up[b][lw * 8 + t] = on ? __uint_as_float(static_cast<uint32_t>(eb) << 23) : 0.f;
-      sm.tok_dn[b][lw * 8 + t] = on ? dn : 0.f;
-    }
-    if (next) load_token<kFp4, kBlocks>(p, *next, lw, lane, t, r);
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int t = 4 * i + (lane >> 3);
-    const float f = __uint_as_float(static_cast<uint32_t>(254 - eb_rope[i]) << 23) * (1.f / (1 << kRopeShift));
-    st_shared_v4(base + 8 * kChunkBytes + t * 128 + (((lane & 7) ^ t) << 4), bf2_to_h2(r.rope[i].x, f),
-                 bf2_to_h2(r.rope[i].y, f), bf2_to_h2(r.rope[i].z, f), bf2_to_h2(r.rope[i].w, f));
-  }
-  if (next) load_rope<kFp4, kBlocks>(p, *next, lw, lane, r);
+    st_shared_v4<i * kChunk>(p0, y[0], y[1], y[2], y[3]);
+    st_shared_v4<i * kChunk>(p1, y[4], y[5], y[6], y[7]);
+  });
 }
 
+// Walks the tiles of a CTA's range.
+struct Walk {
+  int64_t row;
+  int hg, tile, seg;  // seg: jobs since the first
+  __device__ __forceinline__ Walk(const AttnArgs& p, int64_t job, int t)
+      : row(job / p.n_hg), hg(static_cast<int>(job % p.n_hg)), tile(t), seg(0) {}
+  __device__ __forceinline__ void next(const AttnArgs& p) {
+    if (++tile == p.tiles) {
+      tile = 0;
+      next_job(p);
+    }
+  }
+  __device__ __forceinline__ void next_job(const AttnArgs& p) {
+    ++seg;
+    if (++hg == p.n_hg) {
+      hg = 0;
+      ++row;
+    }
+  }
+};
+
 template <bool kFp4, bool kBlocks>
-__global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const AttnArgs p) {
+__global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_constant__ CUtensorMap map,
+                                                                    const AttnArgs p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   AtSmem& sm = smem_aligned_1024<AtSmem>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -429,12 +564,15 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const AttnArg
       mbar_init(&sm.sfull[i], 1);
       mbar_init(&sm.pready[i], kSoftWarps);
     }
-    mbar_init(&sm.qfull, kLoadWarps);
+    mbar_init(&sm.rfull, 1);
+    mbar_init(&sm.rempty, kLoadWarps);
+    mbar_init(&sm.qfull, kQWarps);
     mbar_init(&sm.qempty, 1);
     mbar_init(&sm.oempty, kSoftWarps);
     mbar_init(&sm.done, 1);
     sm.abort = 0;
     fence_barrier_init();
+    tma_prefetch_desc(&map);
   }
   if (warp == kMmaWarp) {
     tmem_alloc(&sm.tmem, kTmemCols);
@@ -445,123 +583,199 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const AttnArg
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
   volatile int* abort = &sm.abort;
+  const uint64_t limit = wait_limit_ns();
 
   // Every role walks the CTA's n tiles; no role leaves early, so that the named barriers of the
   // softmax warps stay complete: after a wait ran out (abort) the remaining waits return at once and
   // no more MMAs are issued.
   if (warp >= kLoadWarp) {
     // ------------------------------------------------ loaders
-    const int lw = warp - kLoadWarp;
-    Raw<kFp4> raw;
-    int64_t job = job0, njob = job0;
-    int tile = tile0, ntile = tile0, seg = 0;
-    Cand cur = candidates<kBlocks>(p, job / p.n_hg, tile, lane), nxt = cur;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) load_token<kFp4, kBlocks>(p, cur, lw, lane, t, raw);
-    load_rope<kFp4, kBlocks>(p, cur, lw, lane, raw);
+    const int lw = warp - kLoadWarp, tok = lw * 8 + (lane >> 2);
+    const uint32_t mine = smem_u32(sm.raw) + tok * (kFp4 ? kRawFp4 : kRawFp8);
+    int tile = tile0, seg = 0;
     for (int g = 0; g < n; ++g) {
       const int b = g & 1;
-      const bool more = g + 1 < n;
-      if (more) {
-        if (++ntile == p.tiles) {
-          ntile = 0;
-          ++njob;
-        }
-        nxt = candidates<kBlocks>(p, njob / p.n_hg, ntile, lane);
-      }
-      const bool first = g == 0 || tile == 0;
-      float cq = 0.f;
-      if (first) {
-        if (seg > 0) mbar_wait(&sm.qempty, (seg - 1) & 1, abort, &g_hcu_status);
-        ++seg;
-        cq = load_q(p, sm, job / p.n_hg, static_cast<int>(job % p.n_hg) * kHg, lw, lane);
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.qfull);
-      }
+      mbar_wait(&sm.rfull, g & 1, abort, &g_hcu_status);
+      const uint32_t m0 = sm.mask[0], m1 = sm.mask[1];
+      const bool some = (m0 | m1) != 0;
+      const bool on = (tok < 32 ? m0 >> tok : m1 >> (tok - 32)) & 1;
+      Raw<kFp4> raw;
+      if (some) read_raw<kFp4>(mine, lane & 3, raw);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.rempty);
       if (g >= 2) mbar_wait(&sm.empty[b], ((g >> 1) - 1) & 1, abort, &g_hcu_status);
-      if (first && (lane & 3) == 0) sm.cq[b][lw * 8 + (lane >> 2)] = cq;
-      if (cur.any) {
-        store_tile<kFp4, kBlocks>(p, sm, b, cur, more ? &nxt : nullptr, lw, lane, raw);
+      if (some) {
+        store_tile<kFp4>(sm, b, lw, lane, on, raw);
         fence_async_shared();
-      } else if (more) {
-#pragma unroll
-        for (int t = 0; t < 8; ++t) load_token<kFp4, kBlocks>(p, nxt, lw, lane, t, raw);
-        load_rope<kFp4, kBlocks>(p, nxt, lw, lane, raw);
       }
-      if (lw == 0 && lane == 0) sm.empty_tile[b] = !cur.any;
+      if (lw == 0) {
+        // the softmax warps read the segment's cq after this tile's `full`: pass the Q warps' writes on
+        if (g == 0 || tile == 0) mbar_wait(&sm.qfull, (seg++) & 1, abort, &g_hcu_status);
+        if (lane == 0) sm.empty_tile[b] = !some;
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.full[b]);
-      cur = nxt;
-      job = njob;
-      tile = ntile;
+      if (++tile == p.tiles) tile = 0;
     }
+  } else if (warp == kGatherWarp) {
+    // ------------------------------------------------ gather: slots into the raw buffer
+    constexpr int stride = kFp4 ? kRawFp4 : kRawFp8;
+    const uint32_t dst = smem_u32(sm.raw) + 4 * lane * stride;
+    int last_copies = -1;  // the last tile that has copies
+    Walk ahead(p, job0, tile0), at = ahead;  // `ahead` names the tile whose entries are fetched next, `at` the place's
+    Entry entry = load_entry<kBlocks>(p, ahead.row, ahead.tile, lane, true);
+    ahead.next(p);
+    Place place = load_place<kBlocks>(p, at.row, at.tile, lane, entry);
+    at.next(p);
+    entry = load_entry<kBlocks>(p, ahead.row, ahead.tile, lane, n > 1);
+    ahead.next(p);
+    for (int g = 0; g < n; ++g) {
+      int32_t s[4];
+      uint32_t has = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[i] = resolve<kBlocks>(p, place, i);
+        has |= s[i] >= 0 ? 1u << i : 0u;
+      }
+      const uint32_t m0 = __reduce_or_sync(0xffffffffu, lane < 8 ? has << (4 * lane) : 0u);
+      const uint32_t m1 = __reduce_or_sync(0xffffffffu, lane >= 8 && lane < kGatherLanes ? has << (4 * (lane - 8)) : 0u);
+      place = load_place<kBlocks>(p, at.row, at.tile, lane, entry);
+      at.next(p);
+      entry = load_entry<kBlocks>(p, ahead.row, ahead.tile, lane, g + 2 < n);
+      ahead.next(p);
+      // a wait that ran out: no more copies (their barrier phases could no longer be told apart)
+      if (g > 0 && !mbar_wait(&sm.rempty, (g - 1) & 1, abort, &g_hcu_status)) break;
+      const bool some = (m0 | m1) != 0;
+      if (lane == 0) {
+        sm.mask[0] = m0;
+        sm.mask[1] = m1;
+        if (some)
+          mbar_arrive_expect_tx(&sm.rfull, kTile * stride);
+        else
+          mbar_arrive(&sm.rfull);
+      }
+      __syncwarp();
+      if (some) {
+        if (lane < kGatherLanes) tma_gather4(dst, &map, &sm.rfull, s[0], s[1], s[2], s[3]);
+        last_copies = g;
+      }
+      __syncwarp();
+    }
+    // copies in flight must land before the CTA may exit
+    if (last_copies >= 0 && *abort) mbar_wait_drain(&sm.rfull, last_copies & 1, &g_hcu_status);
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------ MMA issuer
     if (elect_one()) {
+      // The first product of tile s and the second of tile o, whichever has its operands: the second
+      // must not wait for a later tile's slots (its buffer is what they are waiting for), nor the
+      // first for the softmax in between.  S has two buffers, so s runs at most two tiles ahead of o.
       constexpr uint32_t id_s = idesc_f16(64, kTile, false);
-      int64_t job = job0;
-      int tile = tile0, seg = -1;
-      bool prev_empty = true, prev_first = false;  // of the tile whose second product is due
-      int prev_seg = 0, prev_n = kHg;
-      uint32_t acc = 0;  // the segment's O holds something
-      const auto second = [&](int h) {  // O^T += V^T P^T of tile h
-        const int b = h & 1;
-        if (prev_first) acc = 0;
-        bool ok = mbar_wait(&sm.pready[b], (h >> 1) & 1, abort, &g_hcu_status);
-        if (prev_empty) {
-          mbar_arrive(&sm.empty[b]);
-          return;
-        }
-        if (acc == 0 && prev_seg > 0) ok = mbar_wait(&sm.oempty, (prev_seg - 1) & 1, abort, &g_hcu_status) && ok;
-        tc_fence_after();
-        if (ok && !*abort) {
-          const uint32_t id_o = idesc_f16(128, prev_n, true);
-          const uint64_t v = sw128_mnmajor_desc(smem_u32(sm.k[b]));
-          const uint64_t pd = sw128_kmajor_desc(smem_u32(sm.k[b]) + 8 * kChunkBytes);
+      int s = 0, o = 0;                                      // tiles of the CTA's range
+      int s_tile = tile0, s_seg = 0, o_tile = tile0, o_seg = 0;  // their places in their jobs
+      int o_hg = static_cast<int>(job0 % p.n_hg);
+      uint32_t s_none = 0;  // bit b: the tile in buffer b holds no token
+      uint32_t acc = 0;     // the segment's O holds something
+      bool q_ok = false;    // the segment's Q has been waited for
+      uint64_t t0 = 0;
+      while (o < n) {
+        bool moved = false;
+        if (s < n && s < o + 2) {
+          const int b = s & 1;
+          if (!q_ok) q_ok = mbar_test(&sm.qfull, s_seg & 1);
+          if (q_ok && mbar_test(&sm.full[b], (s >> 1) & 1)) {
+            moved = true;
+            tc_fence_after();
+            s_none &= ~(1u << b);
+            if (!sm.empty_tile[b]) {
+              const uint64_t qd = sw128_kmajor_desc(smem_u32(sm.q)), kd = sw128_kmajor_desc(smem_u32(sm.k[b]));
 #pragma unroll
-          for (int ks = 0; ks < kTile / 16; ++ks)
-#pragma unroll
-            for (int d = 0; d < 4; ++d)
-              mma_f16(tmem + kTmemO + 64 * d, v + ((2 * d * kChunkBytes + ks * 2048) >> 4), pd + 2 * ks, id_o,
-                      ks > 0 ? 1u : acc);
-        }
-        acc = 1;
-        tc_commit(&sm.empty[b]);
-      };
-      for (int g = 0; g < n; ++g) {
-        const int b = g & 1;
-        const bool first = g == 0 || tile == 0;
-        const bool last = tile + 1 == p.tiles;  // of the job; the CTA's last segment needs no release
-        if (first) mbar_wait(&sm.qfull, (++seg) & 1, abort, &g_hcu_status);
-        const bool ok = mbar_wait(&sm.full[b], (g >> 1) & 1, abort, &g_hcu_status);
-        const bool none = !ok || sm.empty_tile[b];
-        tc_fence_after();
-        if (!none) {
-          const uint64_t qd = sw128_kmajor_desc(smem_u32(sm.q)), kd = sw128_kmajor_desc(smem_u32(sm.k[b]));
-#pragma unroll
-          for (int k = 0; k < kQkDim / 16; ++k) {
-            const uint32_t off = ((k >> 2) * kChunkBytes + (k & 3) * 32) >> 4;
-            mma_f16(tmem + kTmemS + 64 * b, qd + off, kd + off, id_s, k > 0 ? 1u : 0u);
+              for (int k = 0; k < kQkDim / 16; ++k) {
+                const uint32_t c = k >> 2, off = (k & 3) * 32;
+                mma_f16(tmem + kTmemS + 64 * b, qd + ((c * kQChunk + off) >> 4), kd + ((c * kChunk + off) >> 4), id_s,
+                        k > 0 ? 1u : 0u);
+              }
+              tc_commit(&sm.sfull[b]);
+            } else {
+              s_none |= 1u << b;
+              mbar_arrive(&sm.sfull[b]);
+            }
+            ++s;
+            if (++s_tile == p.tiles) {
+              tc_commit(&sm.qempty);  // the job's last product with this Q
+              s_tile = 0;
+              ++s_seg;
+              q_ok = false;
+            }
           }
-          tc_commit(&sm.sfull[b]);
-        } else {
-          mbar_arrive(&sm.sfull[b]);
         }
-        if (last) tc_commit(&sm.qempty);
-        if (g > 0) second(g - 1);
-        prev_empty = none;
-        prev_first = first;
-        prev_seg = seg;
-        prev_n = (min(kHg, p.heads - static_cast<int>(job % p.n_hg) * kHg) + 15) & ~15;
-        if (++tile == p.tiles) {
-          tile = 0;
-          ++job;
+        if (o < s) {
+          const int b = o & 1;
+          const bool none = s_none >> b & 1;
+          if (o == 0 || o_tile == 0) acc = 0;
+          // a segment's first product overwrites O: the output of the segment before must be done
+          if (mbar_test(&sm.pready[b], (o >> 1) & 1) &&
+              (none || acc != 0 || o_seg == 0 || mbar_test(&sm.oempty, (o_seg - 1) & 1))) {
+            moved = true;
+            if (none) {
+              mbar_arrive(&sm.empty[b]);
+            } else {
+              tc_fence_after();
+              const uint32_t id_o = idesc_f16(128, (min(kHg, p.heads - o_hg * kHg) + 15) & ~15, true);
+              const uint64_t v = sw128_mnmajor_desc(smem_u32(sm.k[b]));
+              const uint64_t pd = sw32_kmajor_desc(smem_u32(sm.k[b]) + 8 * kChunk);
+#pragma unroll
+              for (int ks = 0; ks < kTile / 16; ++ks)
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                  mma_f16(tmem + kTmemO + 64 * d, v + ((2 * d * kChunk + ks * 2048) >> 4), pd + ((ks * 2048) >> 4), id_o,
+                          ks > 0 ? 1u : acc);
+              acc = 1;
+              tc_commit(&sm.empty[b]);
+            }
+            ++o;
+            if (++o_tile == p.tiles) {
+              o_tile = 0;
+              ++o_seg;
+              if (++o_hg == p.n_hg) o_hg = 0;
+            }
+          }
+        }
+        if (moved) {
+          t0 = 0;
+        } else {
+          if (t0 == 0) t0 = globaltimer();
+          if (*abort || globaltimer() - t0 > limit) {  // nothing became ready for too long: give up
+            if (!*abort) atomicOr(&g_hcu_status, HCU_STATUS_WAIT_TIMEOUT);
+            *abort = 1;
+            break;
+          }
         }
       }
-      second(n - 1);
       tc_commit(&sm.done);
       mbar_wait_drain(&sm.done, 0, &g_hcu_status);
+    }
+  } else if (warp >= kQWarp) {
+    // ------------------------------------------------ queries
+    // Q is single-buffered: the next segment's rows are brought into L2 while this one's are in use.
+    // Four cq buffers: when a segment's Q is released, its second predecessor's first tile is done with.
+    const int qw = warp - kQWarp;
+    Walk at(p, job0, 0);
+    const int segs = (tile0 + n + p.tiles - 1) / p.tiles;
+    for (int seg = 0; seg < segs; ++seg) {
+      if (seg > 0) mbar_wait(&sm.qempty, (seg - 1) & 1, abort, &g_hcu_status);
+#pragma unroll 1
+      for (int hp = qw; hp < kHg / 8; hp += kQWarps) load_q(p, sm, sm.cq[seg & 3], at.row, at.hg * kHg, hp, lane);
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.qfull);
+      at.next_job(p);
+      if (seg + 1 < segs) {
+        for (int h = qw * 32 + lane; h < kHg * 9; h += kQWarps * 32) {  // 9 lines of 128 bytes per head
+          const int hd = at.hg * kHg + h / 9;
+          if (hd < p.heads)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(p.q + at.row * p.q_row + hd * p.q_head + 64 * (h % 9)));
+        }
+      }
     }
   } else {
     // ------------------------------------------------ softmax and output
@@ -579,8 +793,8 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const AttnArg
       if (g == 0 || tile == 0) {
         m0 = m1 = -INFINITY;
         l0 = l1 = 0.f;
-        cq0 = sm.cq[b][r0];
-        cq1 = sm.cq[b][r1];
+        cq0 = sm.cq[seg & 3][r0];
+        cq1 = sm.cq[seg & 3][r1];
         started = false;
       }
       const bool none = sm.empty_tile[b] || *abort;
@@ -590,11 +804,11 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const AttnArg
         if (lane == 0) mbar_arrive(&sm.pready[b]);
       } else {
         tc_fence_after();
-        uint32_t s[32];
-        tmem_ld_16x256_x8(tmem + kTmemS + 64 * b + quad, s);
+        uint32_t s[24];
+        tmem_ld_scores(tmem + kTmemS + 64 * b + quad, s);
         float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 6; ++i) {
           const float2 up = *reinterpret_cast<const float2*>(&sm.tok_up[b][8 * i + cl]);
           const float2 e = *reinterpret_cast<const float2*>(&sm.tok_e[b][8 * i + cl]);
           const float w0 = fmaf(__uint_as_float(s[4 * i]) * up.x, cq0, e.x);
@@ -648,10 +862,11 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const AttnArg
           }
         }
         const float b0 = m0 == -INFINITY ? 0.f : m0 - kBias, b1 = m1 == -INFINITY ? 0.f : m1 - kBias;
-        const uint32_t pbase = smem_u32(sm.k[b]) + 8 * kChunkBytes + warp * 2048 + ((lane >> 3) & 1) * 1024 +
-                               (lane & 7) * 128;
+        // P: for every 16 tokens [64 heads][16 tokens], rows of 32 bytes with the 32-byte swizzle
+        const int ph = 16 * warp + 8 * ((lane >> 3) & 1) + (lane & 7);
+        const uint32_t pdst = smem_u32(sm.k[b]) + 8 * kChunk + st_piece(ph, lane >> 4);
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
+        for (int i = 0; i < 6; i += 2) {
           uint32_t h[4];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
@@ -667,8 +882,7 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const AttnArg
             h[2 * k + 1] = h2_bits(__floats2half2_rn(p2, p3));
           }
           // matrices: (tokens 8 i.., heads r0), (.., heads r1), (tokens 8 (i + 1).., heads r0), (.., r1)
-          const int unit = i + (lane >> 4);
-          stmatrix_x4(pbase + ((unit ^ (lane & 7)) << 4), h[0], h[1], h[2], h[3]);
+          stmatrix_x4(pdst + i * 1024, h[0], h[1], h[2], h[3]);
         }
         started = true;
         fence_async_shared();
@@ -706,38 +920,63 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const AttnArg
         mbar_wait(&sm.empty[b], (g >> 1) & 1, abort, &g_hcu_status);  // the last product is complete
         named_bar(2, kSoftWarps * 32);
         tc_fence_after();
+        if (whole) {
+          // 16 latent values x 32 heads at a time: fragments, transposed into the warp's 1 KB as rows of
+          // 32 bytes per head, then stored as whole sectors
+          const uint32_t st = smem_u32(sm.stage[warp]);
+          uint16_t* dst = p.out + (row * p.heads + h0) * kLatentDim + 32 * warp + 8 * (lane & 1);
+          const int piece = st_piece(lane >> 1, lane & 1);
 #pragma unroll 1
-        for (int c = 0; c < 8; ++c) {  // 32 heads of 128 latent values
-          const int hb = 32 * (c & 1);
-          if (hb >= nh) continue;
-          const int d = 128 * (c >> 1) + 32 * warp + lane;
-          uint32_t o[32];
-          if (started) {
-            tmem_ld_x32_sync(tmem + kTmemO + quad + 32 * c, o);
-          } else {
+          for (int hb = 0; hb < nh; hb += 32) {
+            float2 f[4];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = 0;
-          }
-          const float4* f4 = reinterpret_cast<const float4*>(sm.factor + hb);
-          if (whole) {
-            // neighbouring lanes trade halves: each stores two adjacent values of one head
-            uint16_t* dst = p.out + ((row * p.heads + h0 + hb + (lane & 1)) * kLatentDim + (d & ~1));
+            for (int i = 0; i < 4; ++i) f[i] = *reinterpret_cast<const float2*>(&sm.factor[hb + 8 * i + cl]);
+#pragma unroll 2
+            for (int c = 0; c < 8; ++c) {  // latent values 128 (c / 2) + 32 warp + 16 (c % 2) ..
+              uint32_t o[16];
+              if (started) {
+                tmem_ld_16x256_x4(tmem + kTmemO + 64 * (c >> 1) + hb + quad + (static_cast<uint32_t>(16 * (c & 1)) << 16),
+                                  o);
+              } else {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 f = f4[j / 4];
-              const float v0 = __uint_as_float(o[j]) * f.x, v1 = __uint_as_float(o[j + 1]) * f.y;
-              const float v2 = __uint_as_float(o[j + 2]) * f.z, v3 = __uint_as_float(o[j + 3]) * f.w;
-              const float t0 = __shfl_xor_sync(0xffffffffu, lane & 1 ? v0 : v1, 1);
-              const float t1 = __shfl_xor_sync(0xffffffffu, lane & 1 ? v2 : v3, 1);
-              const __nv_bfloat162 w0 = lane & 1 ? __floats2bfloat162_rn(t0, v1) : __floats2bfloat162_rn(v0, t0);
-              const __nv_bfloat162 w1 = lane & 1 ? __floats2bfloat162_rn(t1, v3) : __floats2bfloat162_rn(v2, t1);
-              if (hb + j + (lane & 1) < nh)
-                *reinterpret_cast<__nv_bfloat162*>(dst + static_cast<int64_t>(j) * kLatentDim) = w0;
-              if (hb + j + 2 + (lane & 1) < nh)
-                *reinterpret_cast<__nv_bfloat162*>(dst + static_cast<int64_t>(j + 2) * kLatentDim) = w1;
+                for (int j = 0; j < 16; ++j) o[j] = 0;
+              }
+              uint32_t w[8];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(__uint_as_float(o[4 * i]) * f[i].x,
+                                                                __uint_as_float(o[4 * i + 1]) * f[i].y);
+                const __nv_bfloat162 hi = __floats2bfloat162_rn(__uint_as_float(o[4 * i + 2]) * f[i].x,
+                                                                __uint_as_float(o[4 * i + 3]) * f[i].y);
+                w[2 * i] = *reinterpret_cast<const uint32_t*>(&lo);
+                w[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+              }
+              // matrices: (values 0-7, heads 8 i ..), (values 8-15, heads 8 i ..), then heads 8 (i + 1) ..
+              const int hr = 8 * (lane >> 4) + (lane & 7), part = (lane >> 3) & 1;
+              stmatrix_x4_trans(st + st_piece(hr, part), w[0], w[1], w[2], w[3]);
+              stmatrix_x4_trans(st + st_piece(hr + 16, part), w[4], w[5], w[6], w[7]);
+              __syncwarp();
+              const uint4 a0 = ld_shared_v4(st + piece), a1 = ld_shared_v4(st + piece + 16 * 32);
+              uint16_t* d0 = dst + 128 * (c >> 1) + 16 * (c & 1) + static_cast<int64_t>(hb + (lane >> 1)) * kLatentDim;
+              if (hb + (lane >> 1) < nh) *reinterpret_cast<uint4*>(d0) = a0;
+              if (hb + (lane >> 1) + 16 < nh) *reinterpret_cast<uint4*>(d0 + 16 * kLatentDim) = a1;
+              __syncwarp();
             }
-          } else {
-            float* dst = part + hb * kLatentDim + d;
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {  // 32 heads of 128 latent values
+            const int hb = 32 * (c & 1);
+            if (hb >= nh) continue;
+            uint32_t o[32];
+            if (started) {
+              tmem_ld_x32_sync(tmem + kTmemO + quad + 32 * c, o);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = 0;
+            }
+            const float4* f4 = reinterpret_cast<const float4*>(sm.factor + hb);
+            float* dst = part + hb * kLatentDim + 128 * (c >> 1) + 32 * warp + lane;
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
               const float4 f = f4[j / 4];
@@ -814,15 +1053,45 @@ int attn_grid(int64_t total) {
 
 int64_t tiles_of(int64_t n_tokens) { return n_tokens <= 0 ? 1 : (n_tokens + kTile - 1) / kTile; }
 
+// The cache as rows of 4-byte words (a slot's words; the box is one row, padded to the raw stride).
+int slot_map(CUtensorMap* m, const AttnArgs& a, bool fp4) {
+  static std::once_flag once;
+  static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+  std::call_once(once, [] {
+    cudaDriverEntryPointQueryResult q;
+    void* ptr = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  });
+  // an empty cache: a map that no copy reads (every candidate is out of range)
+  const void* base = a.n_slots > 0 ? static_cast<const void*>(a.kv) : static_cast<const void*>(a.q);
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>((fp4 ? kKv4Slot : kFp8Slot) / 4),
+                              static_cast<cuuint64_t>(a.n_slots > 0 ? a.n_slots : 1)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(a.slot_stride)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>((fp4 ? kRawFp4 : kRawFp8) / 4), 1};
+  const cuuint32_t step[2] = {1, 1};
+  if (!encode || encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+    set_last_error_msg("cuTensorMapEncodeTiled rejected the tensor map of ", "the MLA cache");
+    return HCU_ERR_LAUNCH;
+  }
+  return HCU_OK;
+}
+
 template <bool kFp4, bool kBlocks>
 int launch_attn(const AttnArgs& a, int grid, cudaStream_t st) {
+  CUtensorMap map;
+  const int rc = slot_map(&map, a, kFp4);
+  if (rc != HCU_OK) return rc;
   constexpr int smem = static_cast<int>(sizeof(AtSmem)) + 1024;
   cudaError_t e = cudaFuncSetAttribute(sparse_mla_kernel<kFp4, kBlocks>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
     set_last_error(e);
     return HCU_ERR_LAUNCH;
   }
-  sparse_mla_kernel<kFp4, kBlocks><<<grid, kAtThreads, smem, st>>>(a);
+  sparse_mla_kernel<kFp4, kBlocks><<<grid, kAtThreads, smem, st>>>(map, a);
   bool split = false;
   for (int c = 1; c < grid && !split; ++c) split = (a.total * c / grid) % a.tiles != 0;
   if (split) {
@@ -895,6 +1164,9 @@ extern "C" int hcu_sparse_mla_attention(const uint16_t* q, int64_t rows, int64_t
   a.out = out;
   a.lse = lse;
   a.part = static_cast<float*>(workspace);
+  // an empty list or table is read (its entries dropped) at some valid address
+  if (n_idx == 0) a.idx = reinterpret_cast<const int32_t*>(q), a.idx_stride = 0;
+  if (blocks && n_bt == 0) a.bt = reinterpret_cast<const int32_t*>(q), a.bt_stride = 0;
   const int grid = attn_grid(a.total);
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (fp4) return blocks ? launch_attn<true, true>(a, grid, st) : launch_attn<true, false>(a, grid, st);
