@@ -60,7 +60,7 @@ constexpr int kSoftWarps = 4;
 constexpr int kMmaWarp = kSoftWarps;
 constexpr int kGatherWarp = kMmaWarp + 1;
 constexpr int kQWarp = kGatherWarp + 1;
-constexpr int kQWarps = 3;
+constexpr int kQWarps = 4;
 constexpr int kLoadWarp = kQWarp + kQWarps;
 constexpr int kLoadWarps = kTile / 8;
 constexpr int kAtThreads = (kLoadWarp + kLoadWarps) * 32;
@@ -300,6 +300,13 @@ __device__ __forceinline__ uint32_t ldg_u32(const void* p) {
   asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
   return v;
 }
+// The same rows into L2 only.
+__device__ __forceinline__ void tma_prefetch4(const CUtensorMap* map, int r0, int r1, int r2, int r3) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile::gather4 [%0, {%1, %2, %3, %4, %5}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(0), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
+               : "memory");
+}
 // Asynchronous copy of four slots (rows of the map, one row per box) into consecutive rows of shared
 // memory; a row out of range (-1) and the box's bytes past the slot are filled with zeros.
 __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int r0, int r1, int r2,
@@ -434,18 +441,29 @@ __device__ __forceinline__ int exponent2(__nv_bfloat162 m) {
 
 __device__ __forceinline__ float exp2_of(int biased) { return __uint_as_float(static_cast<uint32_t>(biased) << 23); }
 
-// Heads 8 hp .. 8 hp + 7 of a job into the Q buffer, four lanes each; cq[h] is the head's factor from
-// the product to the score in base 2.
-__device__ __forceinline__ void load_q(const AttnArgs& p, AtSmem& sm, float* cq, int64_t row, int h0, int hp,
-                                       int lane) {
-  const int hr = lane >> 2, sub = lane & 3;
-  const int h = h0 + hp * 8 + hr;
+// Heads 8 hp .. 8 hp + 7 of a job, four lanes each: 18 pieces of 16 bytes a lane straight to their
+// places in the Q buffer as bf16 (copy_q), converted in place once they are there (convert_q).
+// cq[h] is the head's factor from the product to the score in base 2.
+__device__ __forceinline__ uint32_t q_piece(uint32_t base, int hp, int hr, int u) {
+  return base + hp * 1024 + hr * 128 + (u >> 3) * kQChunk + (((u & 7) ^ hr) << 4);
+}
+
+__device__ __forceinline__ void copy_q(const AttnArgs& p, uint32_t q, int64_t row, int h0, int hp, int lane) {
+  const int hr = lane >> 2, sub = lane & 3, h = h0 + hp * 8 + hr;
   // a head past the last reads head 0: rows of S and columns of O are independent, and its are not stored
   const uint4* src = reinterpret_cast<const uint4*>(p.q + row * p.q_row + (h < p.heads ? h * p.q_head : 0));
-  const uint32_t base = smem_u32(sm.q) + hp * 1024 + hr * 128;
+#pragma unroll
+  for (int i = 0; i < 18; ++i)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(q_piece(q, hp, hr, sub + 4 * i)),
+                 "l"(src + sub + 4 * i)
+                 : "memory");
+}
+
+__device__ __forceinline__ void convert_q(const AttnArgs& p, uint32_t q, float* cq, int hp, int lane) {
+  const int hr = lane >> 2, sub = lane & 3;
   uint4 v[18];
 #pragma unroll
-  for (int i = 0; i < 18; ++i) v[i] = ldg_v4(src + sub + 4 * i);
+  for (int i = 0; i < 18; ++i) v[i] = ld_shared_v4(q_piece(q, hp, hr, sub + 4 * i));
   __nv_bfloat162 am = amax8(v[0]);
 #pragma unroll
   for (int i = 1; i < 18; ++i) am = __hmax2(am, amax8(v[i]));
@@ -457,72 +475,78 @@ __device__ __forceinline__ void load_q(const AttnArgs& p, AtSmem& sm, float* cq,
   const float f_rope = exp2_of(254 - eb + 13);  // 2^10 more
 #pragma unroll
   for (int i = 0; i < 18; ++i) {
-    const int u = sub + 4 * i;
     const float f = i < 16 ? f_lat : f_rope;
-    st_shared_v4(base + (u >> 3) * kQChunk + (((u & 7) ^ hr) << 4), bf2_to_h2(v[i].x, f), bf2_to_h2(v[i].y, f),
-                 bf2_to_h2(v[i].z, f), bf2_to_h2(v[i].w, f));
+    st_shared_v4(q_piece(q, hp, hr, sub + 4 * i), bf2_to_h2(v[i].x, f), bf2_to_h2(v[i].y, f), bf2_to_h2(v[i].z, f),
+                 bf2_to_h2(v[i].w, f));
   }
   if (sub == 0) cq[hp * 8 + hr] = p.sm_scale * 1.4426950408889634f * exp2_of(eb - 3);
 }
 
-// Converts the warp's 8 tokens and stores them as rows 8 lw .. 8 lw + 7 of tile buffer b; on: the
-// lane's token exists.
+// A lane's converted share of a tile, held in registers until the tile's buffer is free.
+struct Conv {
+  uint32_t y[8][8];  // latent elements 64 i + 16 sub .. + 15, two f16 a word
+  uint32_t r[8];     // rope
+  int eb;            // biased exponent taken out of the token
+};
+
 template <bool kFp4>
-__device__ __forceinline__ void store_tile(AtSmem& sm, int b, int lw, int lane, bool on, const Raw<kFp4>& r) {
-  const int tok = lane >> 2, sub = lane & 3;
+__device__ __forceinline__ void convert(const Raw<kFp4>& r, int sub, Conv& c) {
   int re = exponent2(__hmax2(amax8(r.rope[0]), amax8(r.rope[1])));
   re = max(re, __shfl_xor_sync(0xffffffffu, re, 1));
   re = max(re, __shfl_xor_sync(0xffffffffu, re, 2));
   uint32_t smax = r.sc.x & 0x7fffffffu;
   if constexpr (!kFp4)
     smax = max(max(smax, r.sc.y & 0x7fffffffu), max(r.sc.z & 0x7fffffffu, r.sc.w & 0x7fffffffu));
-  const int eb = min(max(max(static_cast<int>(smax >> 23), re - 13 - kRopeShift), 27), 247);
-  const float dn = exp2_of(254 - eb);
-  if (sub == 0) {
-    const int t = lw * 8 + tok;
-    sm.tok_e[b][t] = on ? static_cast<float>(eb - 127) : -INFINITY;
-    sm.tok_up[b][t] = on ? exp2_of(eb) : 0.f;
-    sm.tok_dn[b][t] = on ? dn : 0.f;
-  }
-  // 16-byte pieces 2 sub and 2 sub + 1 of the token's row in every chunk
-  const uint32_t p0 = smem_u32(sm.k[b]) + lw * 1024 + tok * 128 + (((2 * sub) ^ tok) << 4), p1 = p0 ^ 16u;
+  c.eb = min(max(max(static_cast<int>(smax >> 23), re - 13 - kRopeShift), 27), 247);
+  const float dn = exp2_of(254 - c.eb);
   const float fr = dn * (1.f / (1 << kRopeShift));
-  st_shared_v4<8 * kChunk>(p0, bf2_to_h2(r.rope[0].x, fr), bf2_to_h2(r.rope[0].y, fr),
-                                bf2_to_h2(r.rope[0].z, fr), bf2_to_h2(r.rope[0].w, fr));
-  st_shared_v4<8 * kChunk>(p1, bf2_to_h2(r.rope[1].x, fr), bf2_to_h2(r.rope[1].y, fr),
-                                bf2_to_h2(r.rope[1].z, fr), bf2_to_h2(r.rope[1].w, fr));
-  __half2 s[8];  // scale of chunk i
-  if constexpr (kFp4) {
-    const float ts = __uint_as_float(r.sc.x) * dn;
-    const uint32_t w[8] = {r.gs[0].x, r.gs[0].y, r.gs[0].z, r.gs[0].w, r.gs[1].x, r.gs[1].y, r.gs[1].z, r.gs[1].w};
+  const uint32_t rw[8] = {r.rope[0].x, r.rope[0].y, r.rope[0].z, r.rope[0].w,
+                          r.rope[1].x, r.rope[1].y, r.rope[1].z, r.rope[1].w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      s[i] = __float2half2_rn(e4m3_to_float(static_cast<uint8_t>(w[i] >> (8 * sub))) * ts);
-  } else {
-    const uint32_t w[4] = {r.sc.x, r.sc.y, r.sc.z, r.sc.w};
+  for (int i = 0; i < 8; ++i) c.r[i] = bf2_to_h2(rw[i], fr);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[2 * i] = s[2 * i + 1] = __float2half2_rn(__uint_as_float(w[i]) * dn);
-  }
-  unroll8([&](auto I) {
-    constexpr int i = decltype(I)::value;
-    uint32_t y[8];
+  for (int i = 0; i < 8; ++i) {
     if constexpr (kFp4) {
+      const uint4 g = r.gs[i >> 2];
+      const uint32_t w = (i & 3) == 0 ? g.x : (i & 3) == 1 ? g.y : (i & 3) == 2 ? g.z : g.w;
+      const __half2 s =
+          __float2half2_rn(e4m3_to_float(static_cast<uint8_t>(w >> (8 * sub))) * (__uint_as_float(r.sc.x) * dn));
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        y[k] = h2_bits(__hmul2(e2m1x2_to_half2((r.y[i].x >> (8 * k)) & 0xff), s[i]));
-        y[4 + k] = h2_bits(__hmul2(e2m1x2_to_half2((r.y[i].y >> (8 * k)) & 0xff), s[i]));
+        c.y[i][k] = h2_bits(__hmul2(e2m1x2_to_half2((r.y[i].x >> (8 * k)) & 0xff), s));
+        c.y[i][4 + k] = h2_bits(__hmul2(e2m1x2_to_half2((r.y[i].y >> (8 * k)) & 0xff), s));
       }
     } else {
+      const uint32_t w = i < 2 ? r.sc.x : i < 4 ? r.sc.y : i < 6 ? r.sc.z : r.sc.w;
+      const __half2 s = __float2half2_rn(__uint_as_float(w) * dn);
       const uint32_t x[4] = {r.x[i].x, r.x[i].y, r.x[i].z, r.x[i].w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        y[2 * k] = h2_bits(__hmul2(e4m3x2_to_half2(x[k] & 0xffffu), s[i]));
-        y[2 * k + 1] = h2_bits(__hmul2(e4m3x2_to_half2(x[k] >> 16), s[i]));
+        c.y[i][2 * k] = h2_bits(__hmul2(e4m3x2_to_half2(x[k] & 0xffffu), s));
+        c.y[i][2 * k + 1] = h2_bits(__hmul2(e4m3x2_to_half2(x[k] >> 16), s));
       }
     }
-    st_shared_v4<i * kChunk>(p0, y[0], y[1], y[2], y[3]);
-    st_shared_v4<i * kChunk>(p1, y[4], y[5], y[6], y[7]);
+  }
+}
+
+// Stores the warp's 8 tokens as rows 8 lw .. 8 lw + 7 of tile buffer b; on: the lane's token exists.
+__device__ __forceinline__ void store_tile(AtSmem& sm, int b, int lw, int lane, bool on, const Conv& c) {
+  const int tok = lane >> 2, sub = lane & 3;
+  if (sub == 0) {
+    const int t = lw * 8 + tok;
+    sm.tok_e[b][t] = on ? static_cast<float>(c.eb - 127) : -INFINITY;
+    sm.tok_up[b][t] = on ? exp2_of(c.eb) : 0.f;
+    sm.tok_dn[b][t] = on ? exp2_of(254 - c.eb) : 0.f;
+  }
+  // 16-byte pieces 2 sub and 2 sub + 1 of the token's row in every chunk
+  const uint32_t p0 = smem_u32(sm.k[b]) + lw * 1024 + tok * 128 + (((2 * sub) ^ tok) << 4), p1 = p0 ^ 16u;
+  unroll8([&](auto I) {
+    constexpr int i = decltype(I)::value;
+    st_shared_v4<i * kChunk>(p0, c.y[i][0], c.y[i][1], c.y[i][2], c.y[i][3]);
+    st_shared_v4<i * kChunk>(p1, c.y[i][4], c.y[i][5], c.y[i][6], c.y[i][7]);
   });
+  st_shared_v4<8 * kChunk>(p0, c.r[0], c.r[1], c.r[2], c.r[3]);
+  st_shared_v4<8 * kChunk>(p1, c.r[4], c.r[5], c.r[6], c.r[7]);
 }
 
 // Walks the tiles of a CTA's range.
@@ -599,13 +623,20 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
       const uint32_t m0 = sm.mask[0], m1 = sm.mask[1];
       const bool some = (m0 | m1) != 0;
       const bool on = (tok < 32 ? m0 >> tok : m1 >> (tok - 32)) & 1;
-      Raw<kFp4> raw;
-      if (some) read_raw<kFp4>(mine, lane & 3, raw);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.rempty);
+      Conv conv;
+      if (some) {
+        Raw<kFp4> raw;
+        read_raw<kFp4>(mine, lane & 3, raw);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.rempty);
+        convert<kFp4>(raw, lane & 3, conv);
+      } else {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.rempty);
+      }
       if (g >= 2) mbar_wait(&sm.empty[b], ((g >> 1) - 1) & 1, abort, &g_hcu_status);
       if (some) {
-        store_tile<kFp4>(sm, b, lw, lane, on, raw);
+        store_tile(sm, b, lw, lane, on, conv);
         fence_async_shared();
       }
       if (lw == 0) {
@@ -622,30 +653,40 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
     constexpr int stride = kFp4 ? kRawFp4 : kRawFp8;
     const uint32_t dst = smem_u32(sm.raw) + 4 * lane * stride;
     int last_copies = -1;  // the last tile that has copies
+    // Three tiles ahead of the copy: a tile's entries are fetched, then its places; once these are there
+    // its slots are brought into L2, so that the copy into the one raw buffer waits for L2, not HBM.
     Walk ahead(p, job0, tile0), at = ahead;  // `ahead` names the tile whose entries are fetched next, `at` the place's
-    Entry entry = load_entry<kBlocks>(p, ahead.row, ahead.tile, lane, true);
+    Entry entry;
+    Place place;
+    int32_t s[4], nx[4];  // slots of tile g, of tile g + 1
+    uint32_t has, hasn = 0;
+    const auto step = [&](int fetch) {  // place -> slots, entry -> place, list -> entry of tile `fetch`
+#pragma unroll
+      for (int i = 0; i < 4; ++i) nx[i] = resolve<kBlocks>(p, place, i);
+      hasn = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) hasn |= nx[i] >= 0 ? 1u << i : 0u;
+      place = load_place<kBlocks>(p, at.row, at.tile, lane, entry);
+      at.next(p);
+      entry = load_entry<kBlocks>(p, ahead.row, ahead.tile, lane, fetch < n);
+      ahead.next(p);
+    };
+    entry = load_entry<kBlocks>(p, ahead.row, ahead.tile, lane, true);
     ahead.next(p);
-    Place place = load_place<kBlocks>(p, at.row, at.tile, lane, entry);
+    place = load_place<kBlocks>(p, at.row, at.tile, lane, entry);
     at.next(p);
     entry = load_entry<kBlocks>(p, ahead.row, ahead.tile, lane, n > 1);
     ahead.next(p);
+    step(2);
     for (int g = 0; g < n; ++g) {
-      int32_t s[4];
-      uint32_t has = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[i] = resolve<kBlocks>(p, place, i);
-        has |= s[i] >= 0 ? 1u << i : 0u;
-      }
+      for (int i = 0; i < 4; ++i) s[i] = nx[i];
+      has = hasn;
       const uint32_t m0 = __reduce_or_sync(0xffffffffu, lane < 8 ? has << (4 * lane) : 0u);
       const uint32_t m1 = __reduce_or_sync(0xffffffffu, lane >= 8 && lane < kGatherLanes ? has << (4 * (lane - 8)) : 0u);
-      place = load_place<kBlocks>(p, at.row, at.tile, lane, entry);
-      at.next(p);
-      entry = load_entry<kBlocks>(p, ahead.row, ahead.tile, lane, g + 2 < n);
-      ahead.next(p);
+      const bool some = (m0 | m1) != 0;
       // a wait that ran out: no more copies (their barrier phases could no longer be told apart)
       if (g > 0 && !mbar_wait(&sm.rempty, (g - 1) & 1, abort, &g_hcu_status)) break;
-      const bool some = (m0 | m1) != 0;
       if (lane == 0) {
         sm.mask[0] = m0;
         sm.mask[1] = m1;
@@ -659,6 +700,8 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
         if (lane < kGatherLanes) tma_gather4(dst, &map, &sm.rfull, s[0], s[1], s[2], s[3]);
         last_copies = g;
       }
+      step(g + 3);
+      if (hasn) tma_prefetch4(&map, nx[0], nx[1], nx[2], nx[3]);
       __syncwarp();
     }
     // copies in flight must land before the CTA may exit
@@ -763,8 +806,12 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
     const int segs = (tile0 + n + p.tiles - 1) / p.tiles;
     for (int seg = 0; seg < segs; ++seg) {
       if (seg > 0) mbar_wait(&sm.qempty, (seg - 1) & 1, abort, &g_hcu_status);
+      const uint32_t q = smem_u32(sm.q);
 #pragma unroll 1
-      for (int hp = qw; hp < kHg / 8; hp += kQWarps) load_q(p, sm, sm.cq[seg & 3], at.row, at.hg * kHg, hp, lane);
+      for (int hp = qw; hp < kHg / 8; hp += kQWarps) copy_q(p, q, at.row, at.hg * kHg, hp, lane);
+      asm volatile("cp.async.wait_all;" ::: "memory");  // each lane converts what it copied
+#pragma unroll 1
+      for (int hp = qw; hp < kHg / 8; hp += kQWarps) convert_q(p, q, sm.cq[seg & 3], hp, lane);
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.qfull);
