@@ -278,13 +278,6 @@ __device__ __forceinline__ bool soft_any(bool p) {
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-__device__ __forceinline__ uint4 ldg_v4(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
 __device__ __forceinline__ uint2 ld_shared_v2(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
@@ -720,6 +713,7 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
       uint32_t acc = 0;     // the segment's O holds something
       bool q_ok = false;    // the segment's Q has been waited for
       uint64_t t0 = 0;
+      int idle = 0;
       while (o < n) {
         bool moved = false;
         if (s < n && s < o + 2) {
@@ -784,9 +778,9 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
           }
         }
         if (moved) {
-          t0 = 0;
-        } else {
-          if (t0 == 0) t0 = globaltimer();
+          idle = 0;
+        } else if ((++idle & 63) == 0) {  // the time is looked at every 64 rounds: a round is on the tile's path
+          if (idle == 64) t0 = globaltimer();
           if (*abort || globaltimer() - t0 > limit) {  // nothing became ready for too long: give up
             if (!*abort) atomicOr(&g_hcu_status, HCU_STATUS_WAIT_TIMEOUT);
             *abort = 1;
@@ -836,7 +830,6 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
     for (int g = 0; g < n; ++g) {
       const int b = g & 1;
       mbar_wait(&sm.full[b], (g >> 1) & 1, abort, &g_hcu_status);  // the loaders' factors and exponents
-      mbar_wait(&sm.sfull[b], (g >> 1) & 1, abort, &g_hcu_status);
       if (g == 0 || tile == 0) {
         m0 = m1 = -INFINITY;
         l0 = l1 = 0.f;
@@ -844,99 +837,103 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
         cq1 = sm.cq[seg & 3][r1];
         started = false;
       }
-      const bool none = sm.empty_tile[b] || *abort;
-      // a wait that ran out leaves the warps with different views: let all of them see the same one
-      if (!soft_any(!none)) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.pready[b]);
-      } else {
+      float2 up[6], e[6], dn[6];  // of the thread's tokens, read while S is computed
+#pragma unroll
+      for (int i = 0; i < 6; ++i) {
+        up[i] = *reinterpret_cast<const float2*>(&sm.tok_up[b][8 * i + cl]);
+        e[i] = *reinterpret_cast<const float2*>(&sm.tok_e[b][8 * i + cl]);
+        dn[i] = *reinterpret_cast<const float2*>(&sm.tok_dn[b][8 * i + cl]);
+      }
+      const bool none = sm.empty_tile[b];
+      mbar_wait(&sm.sfull[b], (g >> 1) & 1, abort, &g_hcu_status);
+      // Every warp goes through the same barriers whatever it saw (after a wait that ran out the warps'
+      // views may differ): one soft_any per tile, and the rescale's two when any warp asks for one.
+      float2 w[12];  // scores in base 2 plus the token's exponent: rows r0 (even), r1 (odd)
+      float mx0 = -INFINITY, mx1 = -INFINITY;
+      if (!none) {
         tc_fence_after();
         uint32_t s[24];
         tmem_ld_scores(tmem + kTmemS + 64 * b + quad, s);
-        float mx0 = -INFINITY, mx1 = -INFINITY;
+        const float2 c0 = make_float2(cq0, cq0), c1 = make_float2(cq1, cq1);
 #pragma unroll
         for (int i = 0; i < 6; ++i) {
-          const float2 up = *reinterpret_cast<const float2*>(&sm.tok_up[b][8 * i + cl]);
-          const float2 e = *reinterpret_cast<const float2*>(&sm.tok_e[b][8 * i + cl]);
-          const float w0 = fmaf(__uint_as_float(s[4 * i]) * up.x, cq0, e.x);
-          const float w1 = fmaf(__uint_as_float(s[4 * i + 1]) * up.y, cq0, e.y);
-          const float w2 = fmaf(__uint_as_float(s[4 * i + 2]) * up.x, cq1, e.x);
-          const float w3 = fmaf(__uint_as_float(s[4 * i + 3]) * up.y, cq1, e.y);
-          mx0 = fmaxf(mx0, fmaxf(w0, w1));
-          mx1 = fmaxf(mx1, fmaxf(w2, w3));
-          s[4 * i] = __float_as_uint(w0);
-          s[4 * i + 1] = __float_as_uint(w1);
-          s[4 * i + 2] = __float_as_uint(w2);
-          s[4 * i + 3] = __float_as_uint(w3);
+          const float2 a = make_float2(__uint_as_float(s[4 * i]), __uint_as_float(s[4 * i + 1]));
+          const float2 d = make_float2(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3]));
+          w[2 * i] = __ffma2_rn(__fmul2_rn(a, up[i]), c0, e[i]);
+          w[2 * i + 1] = __ffma2_rn(__fmul2_rn(d, up[i]), c1, e[i]);
+          mx0 = fmaxf(mx0, fmaxf(w[2 * i].x, w[2 * i].y));
+          mx1 = fmaxf(mx1, fmaxf(w[2 * i + 1].x, w[2 * i + 1].y));
         }
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) {
           mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
           mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
         }
-        if (soft_any(mx0 > m0 + kLazy || mx1 > m1 + kLazy)) {  // m = -inf: any finite maximum
-          const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
-          const float x0 = m0 == n0 ? 1.f : ex2(m0 - n0), x1 = m1 == n1 ? 1.f : ex2(m1 - n1);
-          l0 *= x0;
-          l1 *= x1;
-          m0 = n0;
-          m1 = n1;
-          if (started) {
-            if ((lane & 3) == 0) {
-              sm.factor[r0] = x0;
-              sm.factor[r1] = x1;
-            }
-            mbar_wait(&sm.empty[(g - 1) & 1], ((g - 1) >> 1) & 1, abort, &g_hcu_status);  // O is complete so far
-            named_bar(2, kSoftWarps * 32);
-            tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
-              uint32_t o[32];
-              tmem_ld_x32_sync(tmem + kTmemO + quad + 32 * c, o);
-              const float4* f4 = reinterpret_cast<const float4*>(sm.factor + 32 * (c & 1));
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float4 f = f4[j];
-                o[4 * j] = __float_as_uint(__uint_as_float(o[4 * j]) * f.x);
-                o[4 * j + 1] = __float_as_uint(__uint_as_float(o[4 * j + 1]) * f.y);
-                o[4 * j + 2] = __float_as_uint(__uint_as_float(o[4 * j + 2]) * f.z);
-                o[4 * j + 3] = __float_as_uint(__uint_as_float(o[4 * j + 3]) * f.w);
-              }
-              tmem_st_x32(tmem + kTmemO + quad + 32 * c, o);
-            }
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            named_bar(2, kSoftWarps * 32);  // factor may be written again
-          }
+      }
+      if (soft_any(mx0 > m0 + kLazy || mx1 > m1 + kLazy)) {  // m = -inf: any finite maximum
+        const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+        const float x0 = m0 == n0 ? 1.f : ex2(m0 - n0), x1 = m1 == n1 ? 1.f : ex2(m1 - n1);
+        l0 *= x0;
+        l1 *= x1;
+        m0 = n0;
+        m1 = n1;
+        if ((lane & 3) == 0) {
+          sm.factor[r0] = x0;
+          sm.factor[r1] = x1;
         }
+        if (started) mbar_wait(&sm.empty[(g - 1) & 1], ((g - 1) >> 1) & 1, abort, &g_hcu_status);  // O is complete so far
+        named_bar(2, kSoftWarps * 32);
+        if (started) {
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[32];
+            tmem_ld_x32_sync(tmem + kTmemO + quad + 32 * c, o);
+            const float4* f4 = reinterpret_cast<const float4*>(sm.factor + 32 * (c & 1));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 f = f4[j];
+              o[4 * j] = __float_as_uint(__uint_as_float(o[4 * j]) * f.x);
+              o[4 * j + 1] = __float_as_uint(__uint_as_float(o[4 * j + 1]) * f.y);
+              o[4 * j + 2] = __float_as_uint(__uint_as_float(o[4 * j + 2]) * f.z);
+              o[4 * j + 3] = __float_as_uint(__uint_as_float(o[4 * j + 3]) * f.w);
+            }
+            tmem_st_x32(tmem + kTmemO + quad + 32 * c, o);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+        named_bar(2, kSoftWarps * 32);  // factor may be written again
+      }
+      if (!none) {
         const float b0 = m0 == -INFINITY ? 0.f : m0 - kBias, b1 = m1 == -INFINITY ? 0.f : m1 - kBias;
         // P: for every 16 tokens [64 heads][16 tokens], rows of 32 bytes with the 32-byte swizzle
         const int ph = 16 * warp + 8 * ((lane >> 3) & 1) + (lane & 7);
         const uint32_t pdst = smem_u32(sm.k[b]) + 8 * kChunk + st_piece(ph, lane >> 4);
+        const float2 n0 = make_float2(-b0, -b0), n1 = make_float2(-b1, -b1);
+        float2 z0 = make_float2(l0, 0.f), z1 = make_float2(l1, 0.f);
 #pragma unroll
         for (int i = 0; i < 6; i += 2) {
           uint32_t h[4];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float2 dn = *reinterpret_cast<const float2*>(&sm.tok_dn[b][8 * (i + k) + cl]);
-            const float p0 = ex2(__uint_as_float(s[4 * (i + k)]) - b0), p1 = ex2(__uint_as_float(s[4 * (i + k) + 1]) - b0);
-            const float p2 = ex2(__uint_as_float(s[4 * (i + k) + 2]) - b1),
-                        p3 = ex2(__uint_as_float(s[4 * (i + k) + 3]) - b1);
-            l0 = fmaf(p0, dn.x, l0);
-            l0 = fmaf(p1, dn.y, l0);
-            l1 = fmaf(p2, dn.x, l1);
-            l1 = fmaf(p3, dn.y, l1);
-            h[2 * k] = h2_bits(__floats2half2_rn(p0, p1));
-            h[2 * k + 1] = h2_bits(__floats2half2_rn(p2, p3));
+            const float2 x0 = __fadd2_rn(w[2 * (i + k)], n0), x1 = __fadd2_rn(w[2 * (i + k) + 1], n1);
+            const float2 p0 = make_float2(ex2(x0.x), ex2(x0.y)), p1 = make_float2(ex2(x1.x), ex2(x1.y));
+            z0 = __ffma2_rn(p0, dn[i + k], z0);
+            z1 = __ffma2_rn(p1, dn[i + k], z1);
+            h[2 * k] = h2_bits(__floats2half2_rn(p0.x, p0.y));
+            h[2 * k + 1] = h2_bits(__floats2half2_rn(p1.x, p1.y));
           }
           // matrices: (tokens 8 i.., heads r0), (.., heads r1), (tokens 8 (i + 1).., heads r0), (.., r1)
           stmatrix_x4(pdst + i * 1024, h[0], h[1], h[2], h[3]);
         }
+        l0 = z0.x + z0.y;
+        l1 = z1.x + z1.y;
         started = true;
         fence_async_shared();
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.pready[b]);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.pready[b]);
 
       const bool job_end = tile + 1 == p.tiles;
       if (job_end || g + 1 == n) {
