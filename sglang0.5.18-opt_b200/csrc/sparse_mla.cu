@@ -67,10 +67,12 @@ constexpr int kAtThreads = (kLoadWarp + kLoadWarps) * 32;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kTmemO = 0;    // 4 blocks of 128 latent values x 64 heads
 constexpr uint32_t kTmemS = 256;  // 2 score buffers of 48 columns, 64 apart
-// P is 2^(w - m + kBias): a row's largest weight is 2^11, 2^15 while its maximum has grown by the
-// tolerated 2^kLazy, and weights down to 2^-25 of the largest are normal f16 numbers.
-constexpr float kLazy = 4.f;
-constexpr float kBias = 11.f;
+// P is 2^(w - m + kBias), m the row's maximum when it was last taken: the largest weight is 2^8 then,
+// 2^15 while the maximum has grown by the tolerated 2^kLazy (scores of a row with a spread of 2.2 in
+// base 2 hardly ever rise by 7 over their first 48's maximum), and weights down to 2^-22 of the
+// largest are normal f16 numbers.
+constexpr float kLazy = 7.f;
+constexpr float kBias = 8.f;
 constexpr int kRopeShift = 10;
 constexpr int kPartFloats = kHg * kLatentDim + kHg;
 
@@ -109,12 +111,15 @@ struct AttnArgs {
   int heads, n_hg;
   int tiles;      // per job
   int64_t total;  // jobs * tiles
+  int quantum;    // a CTA's share is a multiple of this many tiles: 1, or a job's
   uint16_t* out;
   float* lse;
   float* part;    // [grid][2][kPartFloats]
 };
 
-__device__ __forceinline__ int64_t first_tile(int64_t total, int cta, int grid) { return total * cta / grid; }
+__host__ __device__ __forceinline__ int64_t first_tile(const AttnArgs& p, int cta, int grid) {
+  return p.total / p.quantum * cta / grid * p.quantum;
+}
 
 // ---------------------------------------------------------------- PTX
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -569,8 +574,8 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   AtSmem& sm = smem_aligned_1024<AtSmem>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t f0 = first_tile(p.total, blockIdx.x, gridDim.x);
-  const int n = static_cast<int>(first_tile(p.total, blockIdx.x + 1, gridDim.x) - f0);  // at least 1
+  const int64_t f0 = first_tile(p, blockIdx.x, gridDim.x);
+  const int n = static_cast<int>(first_tile(p, blockIdx.x + 1, gridDim.x) - f0);  // at least 1
   const int64_t job0 = f0 / p.tiles;
   const int tile0 = static_cast<int>(f0 - job0 * p.tiles);
 
@@ -1052,46 +1057,75 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
 }
 
 // Joins the partial results of a job that several CTAs shared: weights 2^(lse_i - max).  Block
-// (c - 1, h): the job at the boundary between CTAs c - 1 and c, if that is the job's first boundary.
-__global__ __launch_bounds__(128) void combine_kernel(const AttnArgs p, int grid) {
+// (c - 1, y): eight heads of the job at the boundary between CTAs c - 1 and c, if that is the job's first
+// boundary; half a block per head, four latent values a thread.  The partials lie in L2; what the join
+// takes is the latency of its loads, so a head's weights are formed by 128 threads at once and its
+// partials loaded eight at a time.
+constexpr int kCombineThreads = 256, kCombineHeads = 8, kMaxParts = 256;
+
+__global__ __launch_bounds__(kCombineThreads) void combine_kernel(const AttnArgs p, int grid) {
+  __shared__ float weight[2][kMaxParts], red[2][4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x + 1, h = blockIdx.y;
-  const int64_t at = first_tile(p.total, c, grid);
+  const int c = blockIdx.x + 1;
+  const int64_t at = first_tile(p, c, grid);
   const int64_t job = at / p.tiles;
   const int64_t begin = job * p.tiles, end = begin + p.tiles;
-  if (at == begin || first_tile(p.total, c - 1, grid) > begin) return;
+  if (at == begin || first_tile(p, c - 1, grid) > begin) return;
   const int64_t row = job / p.n_hg;
-  const int head = static_cast<int>(job % p.n_hg) * kHg + h;
-  if (head >= p.heads) return;
-  const auto part_of = [&](int cta) {
-    const int slot = first_tile(p.total, cta, grid) / p.tiles == job ? 0 : 1;
-    return p.part + (static_cast<int64_t>(cta) * 2 + slot) * kPartFloats;
-  };
-  float m = -INFINITY;
-  for (int i = c - 1; i < grid && first_tile(p.total, i, grid) < end; ++i)
-    m = fmaxf(m, part_of(i)[kHg * kLatentDim + h]);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  for (int i = c - 1; m != -INFINITY && i < grid && first_tile(p.total, i, grid) < end; ++i) {
-    const float* q = part_of(i);
-    const float w = exp2f(q[kHg * kLatentDim + h] - m);
-    const float4 v = *reinterpret_cast<const float4*>(q + h * kLatentDim + 4 * threadIdx.x);
-    l += w;
-    o.x = fmaf(w, v.x, o.x);
-    o.y = fmaf(w, v.y, o.y);
-    o.z = fmaf(w, v.z, o.z);
-    o.w = fmaf(w, v.w, o.w);
+  const int h0 = static_cast<int>(job % p.n_hg) * kHg;
+  int parts = 1;  // CTAs c - 1 .. c - 2 + parts share the job
+  while (c - 1 + parts < grid && first_tile(p, c - 1 + parts, grid) < end) ++parts;
+  // only the first of them may have started in another job: its part of this one is its second
+  const float* const first = p.part + (static_cast<int64_t>(c - 1) * 2 + (first_tile(p, c - 1, grid) < begin ? 1 : 0)) * kPartFloats;
+  const float* const rest = p.part + static_cast<int64_t>(c) * 2 * kPartFloats;  // of CTA c; CTA c + i: 2 i further
+  const auto part_of = [&](int i) { return i == 0 ? first : rest + static_cast<int64_t>(i - 1) * 2 * kPartFloats; };
+  const int sub = threadIdx.x >> 7, t = threadIdx.x & 127, lane = t & 31;
+#pragma unroll 1
+  for (int it = 0; it < kCombineHeads; it += 2) {
+    const int h = blockIdx.y * kCombineHeads + it + sub;
+    const bool on = h0 + h < p.heads && h < kHg;
+    float lse[kMaxParts / 128], m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kMaxParts / 128; ++k) {
+      const int i = 128 * k + t;
+      lse[k] = on && i < parts ? part_of(i)[kHg * kLatentDim + h] : -INFINITY;
+      m = fmaxf(m, lse[k]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) red[sub][t >> 5] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[sub][0], red[sub][1]), fmaxf(red[sub][2], red[sub][3]));
+#pragma unroll
+    for (int k = 0; k < kMaxParts / 128; ++k)
+      weight[sub][128 * k + t] = m == -INFINITY ? 0.f : exp2f(lse[k] - m);
+    __syncthreads();
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    if (on) {
+#pragma unroll 8
+      for (int i = 0; i < parts; ++i) {
+        const float w = weight[sub][i];
+        const float4 v = *reinterpret_cast<const float4*>(part_of(i) + h * kLatentDim + 4 * t);
+        l += w;
+        o.x = fmaf(w, v.x, o.x);
+        o.y = fmaf(w, v.y, o.y);
+        o.z = fmaf(w, v.z, o.z);
+        o.w = fmaf(w, v.w, o.w);
+      }
+      const float f = l == 0.f ? 0.f : 1.f / l;
+      const __nv_bfloat162 a = __floats2bfloat162_rn(o.x * f, o.y * f), b = __floats2bfloat162_rn(o.z * f, o.w * f);
+      const int64_t rh = row * p.heads + h0 + h;
+      *reinterpret_cast<uint2*>(p.out + rh * kLatentDim + 4 * t) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+      if (t == 0) p.lse[rh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    }
   }
-  const float f = l == 0.f ? 0.f : 1.f / l;
-  const __nv_bfloat162 a = __floats2bfloat162_rn(o.x * f, o.y * f), b = __floats2bfloat162_rn(o.z * f, o.w * f);
-  const int64_t rh = row * p.heads + head;
-  *reinterpret_cast<uint2*>(p.out + rh * kLatentDim + 4 * threadIdx.x) =
-      make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-  if (threadIdx.x == 0) p.lse[rh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
+// CTAs: one per SM at most, and no more than the parts the join holds.
 int attn_grid(int64_t total) {
-  const int64_t sms = sm_count();
+  const int64_t sms = sm_count() < kMaxParts ? sm_count() : kMaxParts;
   return static_cast<int>(total < sms ? total : sms);
 }
 
@@ -1137,11 +1171,12 @@ int launch_attn(const AttnArgs& a, int grid, cudaStream_t st) {
   }
   sparse_mla_kernel<kFp4, kBlocks><<<grid, kAtThreads, smem, st>>>(map, a);
   bool split = false;
-  for (int c = 1; c < grid && !split; ++c) split = (a.total * c / grid) % a.tiles != 0;
+  for (int c = 1; c < grid && !split; ++c) split = first_tile(a, c, grid) % a.tiles != 0;
   if (split) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(grid - 1), static_cast<unsigned>(a.heads < kHg ? a.heads : kHg));
-    cfg.blockDim = dim3(128);
+    const int heads = a.heads < kHg ? a.heads : kHg;
+    cfg.gridDim = dim3(static_cast<unsigned>(grid - 1), static_cast<unsigned>((heads + kCombineHeads - 1) / kCombineHeads));
+    cfg.blockDim = dim3(kCombineThreads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1211,7 +1246,11 @@ extern "C" int hcu_sparse_mla_attention(const uint16_t* q, int64_t rows, int64_t
   // an empty list or table is read (its entries dropped) at some valid address
   if (n_idx == 0) a.idx = reinterpret_cast<const int32_t*>(q), a.idx_stride = 0;
   if (blocks && n_bt == 0) a.bt = reinterpret_cast<const int32_t*>(q), a.bt_stride = 0;
-  const int grid = attn_grid(a.total);
+  // Whole jobs per CTA where that costs less than the join of split ones: sharing a job costs its CTAs
+  // about eight tiles' time (a partial written, read and joined: 128 rows of 43 tiles take 15 us longer split).
+  const int64_t jobs = rows * a.n_hg, sms = attn_grid(a.total);
+  a.quantum = (jobs + sms - 1) / sms * a.tiles <= (a.total + sms - 1) / sms + 8 ? a.tiles : 1;
+  const int grid = static_cast<int>(a.quantum == 1 ? sms : (jobs < sms ? jobs : sms));
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (fp4) return blocks ? launch_attn<true, true>(a, grid, st) : launch_attn<true, false>(a, grid, st);
   return blocks ? launch_attn<false, true>(a, grid, st) : launch_attn<false, false>(a, grid, st);
