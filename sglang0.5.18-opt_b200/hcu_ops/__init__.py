@@ -299,7 +299,7 @@ def step_tables(req_pages, req_idx, seq_lens, new_lens, free_pages, free_head, n
     Request ``i`` of the step is row ``req_idx[i]`` of ``req_pages`` (int32 ``[requests, max_pages]``, page ids
     of 64 tokens), has ``seq_lens[i]`` cached tokens and brings ``new_lens[i]`` new ones (all int32).  The pages
     that the new tokens need come from ``free_pages`` in order, from ``free_head[0]`` on, and are written into
-    ``req_pages`` in place.  The query rows are the new tokens, request by request; ``n_rows`` may exceed their
+    ``req_pages`` in place; the returned ``free_head`` is the next step's.  The query rows are the new tokens, request by request; ``n_rows`` may exceed their
     number (a padded batch): the rows after them are empty (length 0, entries -1).  ``width`` (a multiple of 64)
     is the tokens per row of the tables.  Nothing is read on the host, so a step can be captured in a CUDA graph;
     pages that run out, requests that outgrow the tables and bad lengths give -1 entries and set the device
