@@ -477,7 +477,7 @@ int hcu_select_blocks(const float* score, int64_t rows, int64_t width, int64_t s
  * and saturated; an element stands for code * sg * t.
  *   kv_c  bf16 [n_tokens, 512] row stride kv_tok (16-byte aligned rows), finite
  *   k_pe  bf16 [n_tokens, 64] row stride k_tok (rotated rope, copied)
- *   loc   int64 [n_tokens]; slots out of range are skipped and flagged */
+ *   loc   int64 [n_tokens], distinct; slots out of range are skipped and flagged */
 int hcu_store_mla_kv4(const uint16_t* kv_c, int64_t kv_tok, const uint16_t* k_pe, int64_t k_tok, const int64_t* loc,
                       int64_t n_tokens, uint8_t* kv_buffer, int64_t n_slots, int64_t slot_stride,
                       hcu_stream_t stream);
