@@ -711,10 +711,14 @@ std::vector<torch::Tensor> sparse_mla_attention(const torch::Tensor& q, const to
   const int64_t wsb = hcu_sparse_mla_attention_workspace_bytes(R, H, block_table.has_value() ? 64 * n : n);
   TORCH_CHECK(wsb >= 0, "sparse_mla_attention: bad shape");
   auto ws = torch::empty({wsb}, q.options().dtype(at::kByte));
+  // a table without pages has no address, yet the call is the block form: no entry of it is read
+  const int32_t* table = nullptr;
+  if (block_table.has_value())
+    table = block_table->numel() ? ptr<const int32_t>(*block_table) : reinterpret_cast<const int32_t*>(q.data_ptr());
   check_status(
       hcu_sparse_mla_attention(ptr<const uint16_t>(q), R, H, q.stride(0), q.stride(1), ptr<const uint8_t>(kv_cache),
                                slots, stride, fp4 ? HCU_KV_FP4_432 : HCU_KV_FP8_656, ptr<const int32_t>(indices), n,
-                               indices.stride(0), block_table.has_value() ? ptr<const int32_t>(*block_table) : nullptr,
+                               indices.stride(0), table,
                                block_table.has_value() ? block_table->stride(0) : 0,
                                block_table.has_value() ? block_table->size(1) : 0,
                                lengths.has_value() ? ptr<const int32_t>(*lengths) : nullptr,

@@ -5,22 +5,24 @@
 // over the tokens of the row's list: slots (token form), or the visible tokens of chosen 64-token
 // blocks (block form).
 //
-// Work: a job is (row, group of up to 64 heads), cut into tiles of 64 candidates.  The flat list of
-// all tiles is split evenly over one persistent CTA per SM; a CTA's share of one job is a segment.
-// A segment that is the whole job writes the result, any other one a partial (out, lse) that
-// combine_kernel joins.  Per tile:
-//   * 8 loader warps (one 8-token swizzle group each) gather the slots with 16-byte loads into
-//     registers, convert them to f16 and store them as the tile's K: 9 chunks of [64 tokens][64
-//     values], rows of 128 bytes, 128-byte swizzle.  A chunk is a K-major operand for q k^T and, read
-//     the other way, an MN-major one for v^T, so the latent is stored once.  The next tile's loads go
-//     out as soon as this one is stored;
-//   * 3 warps convert each segment's Q (f16, K-major);
-//   * the MMA thread issues S = Q K^T (M = 64 heads, N = 64 tokens, K = 576) and, up to two tiles
-//     behind, O^T += V^T P^T (M = 128 latent values x 4, N = heads, K = 64 tokens): with the latent as M both
-//     products run without padding rows at 64 heads, and O^T takes 4 x 64 TMEM columns;
+// Work: a job is (row, group of up to 64 heads), cut into tiles of 48 candidates.  The flat list of
+// all tiles is split evenly over one persistent CTA per SM, or job by job where that costs less; a
+// CTA's share of one job is a segment.  A segment that is the whole job writes the result, any other
+// one a partial (out, lse) that combine_kernel joins.  Per tile:
+//   * the gather warp looks the candidates up three tiles ahead, asks their slots into L2 two tiles
+//     ahead, and copies them into the raw buffer, four slots per TMA gather;
+//   * 6 loader warps (one 8-token swizzle group each) read the raw slots, convert them to f16 in
+//     registers, which frees the raw buffer, and store them as the tile's K once a K buffer is free: 9
+//     chunks of [48 tokens][64 values], rows of 128 bytes, 128-byte swizzle.  A chunk is a K-major
+//     operand for q k^T and, read the other way, an MN-major one for v^T, so the latent is stored once;
+//   * 4 warps bring each segment's Q in and convert it in place (f16, K-major);
+//   * the MMA thread issues S = Q K^T (M = 64 heads, N = 48 tokens, K = 576) and, up to two tiles
+//     behind, O^T += V^T P^T (M = 128 latent values x 4, N = heads, K = 48 tokens): with the latent as M
+//     the second product runs at the full rate, and O^T takes 4 x 64 TMEM columns;
 //   * 4 softmax warps (16 heads each) read S, keep the running maximum and sum in fp32 and write P
 //     in f16 over the tile's rope chunk, which S no longer needs.  O^T is rescaled only when a
 //     maximum has risen by more than 2^kLazy.
+// 48 tokens: Q (74 KB), two K tiles (55 KB each) and the raw slots (34 KB) fill the 227 KB.
 //
 // Number format.  f16 operands hold 11 bits where bf16 holds 8, and an fp8 or e2m1 value is exact in
 // f16; its range is met by powers of two taken out per token and per query row:
@@ -32,9 +34,15 @@
 // S * 2^(E + e) is the score; P carries 2^E of its token in its exponent (w = s + E, whose maximum is
 // the running one), so O needs no correction, and the sum takes 2^-E back per token.
 //
-// Bound: at 64 heads the shared-memory port.  A 64-token tile moves 72 KB of K in, 147 KB of Q and K
-// operands for S and 96 KB of V and P for O out: about 2500 cycles at 128 B per cycle, 39 per token,
-// against 24 per token for its products at the dense rate and 15 for its share of HBM.
+// Bound.  A 48-token tile needs 1370 cycles of the tensor pipe (940 for S, whose M of 64 fills half of
+// it, 430 for O) and about 2500 of the shared-memory port at 128 B per cycle (34 KB of raw slots in and out, 55 KB of K in, 126 KB
+// of Q and K operands for S, 72 KB of V and P for O); it takes 3300, 595 tiles a CTA in 1.02 ms for 2048
+// rows x 64 heads x 2048 tokens (584 GFLOP: 573 TFLOP/s).  What is left is the chain of a tile through
+// its warps (copy 2900, convert 650, store 1000, S 940, softmax 1250, O 430 cycles), with two K tiles and
+// one of raw slots to overlap it.  Both were traded: Q partly in TMEM makes room for a third K tile
+// (1.09 ms) or a second raw buffer (1.13 ms), copies of 16 bytes from the loader warps for the raw ring
+// (1.16 to 1.21 ms).  128 rows: 86 us, one row: 24.6 us; 4-bit slots, 192 rows: 137 us (its conversion
+// takes 500 cycles more).  L2 flushed before each call.
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 
@@ -1060,7 +1068,7 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
 // (c - 1, y): two heads of the job at the boundary between CTAs c - 1 and c, if that is the job's first
 // boundary; half a block per head, four latent values a thread.  The partials lie in L2; what the join
 // takes is the latency of its loads, so a head's weights are formed by 128 threads at once and its
-// partials loaded eight at a time.
+// partials loaded eight at a time (one row in 43 parts: the whole call 25 us; with serial loads 52).
 constexpr int kCombineThreads = 256, kCombineHeads = 2, kMaxParts = 256;
 
 __global__ __launch_bounds__(kCombineThreads) void combine_kernel(const AttnArgs p, int grid) {

@@ -11,7 +11,8 @@
 // table and slot table; the last CTA appends the taken pages to req_pages and writes the new head.
 // No CTA reads what another writes: rows take their new pages from free_pages, not from req_pages.
 //
-// Bound: the stores, 4 B per (row, token of width) + 4 B per (row, page).
+// Bound: the stores, 4 B per (row, token of width) + 4 B per (row, page).  128 rows of 65536 tokens (34 MB,
+// 5.3 us at the copy rate of 6.45 TB/s) take 9.4 us in a graph of launches, one row 3.1 us.
 #include "common.cuh"
 
 HCU_DEFINE_STATUS(status_tables)
@@ -20,7 +21,7 @@ namespace hcu {
 namespace {
 
 constexpr int kTbThreads = 256;
-constexpr int kTbPages = 128;  // pages of a row per CTA
+constexpr int kTbPages = 128;  // pages of a row per CTA (128 rows of 65536 tokens: 9.4 us; 64 pages 11.6, 256 pages 9.2)
 
 struct TablesArgs {
   int32_t* req_pages;

@@ -7,7 +7,11 @@ public functions (``sparse_mask_topk_transform``, ``mqa_logits_supported``,
 switches read once at import, and the same hand-off of the fused pass-1
 histogram from ``mqa_logits`` to the next ``sparse_mask_topk_transform``.
 Added: the paged K-cache dequant drop-in, the indexer-K dequant, ragged
-(prefill) logits, top-k with keys and the context-parallel merge.
+(prefill) logits, top-k with keys and the context-parallel merge; and around the
+indexer the step's tables (``step_tables``), the choice of whole blocks
+(``select_blocks``), MLA attention over what was chosen (``sparse_mla_attention``,
+``block_sparse_mla_attention``) and a 4-bit latent cache (``store_mla_kv4``,
+``dequantize_mla_kv4_paged``).
 
 All compute runs in ``libhcu_indexer.so`` (hand-written CUDA for sm_100a)
 behind ``_C``.  There is no fallback: importing this package fails if the

@@ -297,3 +297,20 @@ def test_empty_calls_and_refusals(hcu, dev):
     for t, l in ((i32(3, 4), i32(2)), (i32(2, 4), i32(3)), (i32(2, 4).long(), i32(2))):
         with pytest.raises(RuntimeError):
             hcu.block_sparse_mla_attention(q, P, i32(2, 4), t, l, SCALE)
+
+
+@pytest.mark.parametrize("n", [1, 64])
+def test_table_without_pages_is_still_the_block_form(hcu, dev, n):
+    """A block table of width 0 holds no block: entries below the row's length are flagged, none is a slot."""
+    g = torch.Generator(device=dev)
+    g.manual_seed(3)
+    q = torch.randn(2, 16, 576, generator=g, device=dev).bfloat16()
+    kv = torch.zeros(128, 1, 432, dtype=torch.uint8, device=dev)
+    table = torch.empty(2, 0, dtype=torch.int32, device=dev)
+    blocks = torch.zeros(2, n, dtype=torch.int32, device=dev)
+    hcu.read_device_status()
+    out, lse = hcu.block_sparse_mla_attention(q, kv, blocks, table, torch.full((2,), 64, dtype=torch.int32, device=dev), 0.1)
+    assert (out == 0).all() and (lse == float("-inf")).all()
+    assert hcu.read_device_status() == 2
+    out, lse = hcu.block_sparse_mla_attention(q, kv, blocks, table, torch.zeros(2, dtype=torch.int32, device=dev), 0.1)
+    assert (lse == float("-inf")).all() and hcu.read_device_status() == 0
