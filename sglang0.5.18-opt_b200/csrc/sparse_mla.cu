@@ -633,6 +633,9 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
       if (some) {
         Raw<kFp4> raw;
         read_raw<kFp4>(mine, lane & 3, raw);
+        // The next gather writes these bytes through the async proxy: without the proxy fence it overtook
+        // reads that were still under way (about one row of 2048 tokens x 64 heads in 500 came out wrong).
+        fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.rempty);
         convert<kFp4>(raw, lane & 3, conv);

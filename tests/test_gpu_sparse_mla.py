@@ -314,3 +314,22 @@ def test_table_without_pages_is_still_the_block_form(hcu, dev, n):
     assert hcu.read_device_status() == 2
     out, lse = hcu.block_sparse_mla_attention(q, kv, blocks, table, torch.zeros(2, dtype=torch.int32, device=dev), 0.1)
     assert (lse == float("-inf")).all() and hcu.read_device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "kv4"])
+def test_many_rows_repeat_bit_for_bit(hcu, dev, fmt):
+    """Every SM busy over many tiles: the tile buffers' hand-overs under load.  No atomics, so runs are equal."""
+    rows, pool = 2048, 16384
+    g = torch.Generator(device=dev)
+    g.manual_seed(11)
+    host = _pool(fmt, pool, 11)
+    kv = torch.from_numpy(host).to(dev)
+    q = torch.randn(rows, 64, 576, generator=g, device=dev).bfloat16()
+    idx = torch.randint(0, pool, (rows, 2048), generator=g, device=dev, dtype=torch.int32)
+    out, lse = hcu.sparse_mla_attention(q, kv, idx, SCALE)
+    for _ in range(8):
+        o, z = hcu.sparse_mla_attention(q, kv, idx, SCALE)
+        assert torch.equal(o, out) and torch.equal(z, lse)
+    some = list(range(0, rows, 97))
+    lists = idx[some].cpu().numpy()
+    _check(fmt, q[some].cpu(), host, list(lists), out[some], lse[some])
