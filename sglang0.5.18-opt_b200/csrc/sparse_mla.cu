@@ -31,18 +31,25 @@
 //     rope would leave f16's range (latents 2^-35 below the rope);
 //   * query row: 2^e, its largest element just below 2^4 (latent part) or 2^14 (rope part, which
 //     takes the 2^10 back), so elements down to 2^-18 of the largest keep all their bits.
+// What is rounded, then, is an fp8 value times its scale's mantissa, once in the factor and once in the
+// product; 4-bit values are exact.  Over many tokens the scores' errors of 5e-4 average out (lse of 2048
+// tokens is 4e-6 of itself off, out less than its own bf16 rounding), over few they do not (33 tokens:
+// 5e-5).  A row of few tokens has them in its first tiles, so the first two tiles of a job multiply Q with
+// what the rounding left out as well: lse is off by 7e-7 of itself up to 96 tokens and 1e-5 at most
+// beyond (200 tokens).
+//
 // S * 2^(E + e) is the score; P carries 2^E of its token in its exponent (w = s + E, whose maximum is
 // the running one), so O needs no correction, and the sum takes 2^-E back per token.
 //
 // Bound.  A 48-token tile needs 1370 cycles of the tensor pipe (940 for S, whose M of 64 fills half of
-// it, 430 for O) and about 2500 of the shared-memory port at 128 B per cycle (34 KB of raw slots in and out, 55 KB of K in, 126 KB
-// of Q and K operands for S, 72 KB of V and P for O); it takes 3300, 595 tiles a CTA in 1.02 ms for 2048
-// rows x 64 heads x 2048 tokens (584 GFLOP: 573 TFLOP/s).  What is left is the chain of a tile through
-// its warps (copy 2900, convert 650, store 1000, S 940, softmax 1250, O 430 cycles), with two K tiles and
-// one of raw slots to overlap it.  Both were traded: Q partly in TMEM makes room for a third K tile
-// (1.09 ms) or a second raw buffer (1.13 ms), copies of 16 bytes from the loader warps for the raw ring
-// (1.16 to 1.21 ms).  128 rows: 86 us, one row: 24.6 us; 4-bit slots, 192 rows: 137 us (its conversion
-// takes 500 cycles more).  L2 flushed before each call.
+// it, 430 for O) and about 2500 of the shared-memory port at 128 B per cycle (34 KB of raw slots in and
+// out, 55 KB of K in, 126 KB of Q and K operands for S, 72 KB of V and P for O); it takes 3300.  What is
+// left is the chain of a tile through its warps (copy 2900, convert 650, store 1000, S 940, softmax
+// 1250, O 430 cycles), with two K tiles and one of raw slots to overlap it.  Both were traded: Q partly
+// in TMEM makes room for a third K tile (7 % slower) or a second raw buffer (11 %), copies of 16 bytes from
+// the loader warps replace the raw ring (14 to 19 %).  2048 rows x 64 heads x 2048 fp8 tokens (584 GFLOP)
+// take 1.085 ms, 538 TFLOP/s; 128 rows 91 us; one row 27 us; 192 rows of 4-bit slots 138 us (no
+// remainders, a conversion 500 cycles longer).  L2 flushed before each call.
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 
@@ -82,6 +89,10 @@ constexpr uint32_t kTmemS = 256;  // 2 score buffers of 48 columns, 64 apart
 constexpr float kLazy = 7.f;
 constexpr float kBias = 8.f;
 constexpr int kRopeShift = 10;
+// Tiles at a job's start whose fp8 values are multiplied with their rounding's remainder too (see the
+// number format): 2048 rows x 64 heads x 2048 tokens take 1.085 ms with two of them, 1.015 without any.
+// One leaves lse of 130 to 200 tokens at the edge of 2e-5 of itself.
+constexpr int kFineTiles = 2;
 constexpr int kPartFloats = kHg * kLatentDim + kHg;
 
 struct __align__(1024) AtSmem {
@@ -97,7 +108,7 @@ struct __align__(1024) AtSmem {
   uint32_t mask[2];         // candidates in raw that are tokens
   int empty_tile[2];        // the tile in buffer b holds no token
   uint64_t full[2], empty[2], sfull[2], pready[2];
-  uint64_t rfull, rempty, qfull, qempty, oempty, done;
+  uint64_t rfull, rempty, lfull, lempty, qfull, qempty, oempty, done;
   uint32_t tmem;
   int abort;
 };
@@ -555,6 +566,36 @@ __device__ __forceinline__ void store_tile(AtSmem& sm, int b, int lw, int lane, 
   st_shared_v4<8 * kChunk>(p1, c.r[4], c.r[5], c.r[6], c.r[7]);
 }
 
+// The remainders of the warp's 8 tokens, fp8 value * scale - what store_tile stored, as rows of buffer b.
+// Unscaled: below f16's normal range they lose bits that are 2^-24 of a latent of 1, where the largest
+// is 2^8 to 2^10.
+__device__ __forceinline__ void store_rest(AtSmem& sm, int b, int lw, int lane, uint32_t row, int eb) {
+  const int tok = lane >> 2, sub = lane & 3;
+  const uint32_t p0 = smem_u32(sm.k[b]) + lw * 1024 + tok * 128 + (((2 * sub) ^ tok) << 4), p1 = p0 ^ 16u;
+  const float dn = exp2_of(254 - eb);
+#pragma unroll 2
+  for (int i = 0; i < 8; ++i) {
+    const uint4 x = ld_shared_v4(row + 64 * i + 16 * sub);
+    const float f = __uint_as_float(ld_shared_u32(row + kFp8Scales + 4 * (i >> 1))) * dn;
+    const __half2 s = __float2half2_rn(f);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const __half2 c = e4m3x2_to_half2(w[k >> 1] >> (16 * (k & 1)) & 0xffffu);
+      const float2 v = __half22float2(c), hi = __half22float2(__hmul2(c, s));
+      y[k] = h2_bits(__floats2half2_rn(fmaf(v.x, f, -hi.x), fmaf(v.y, f, -hi.y)));
+    }
+    st_shared_v4(p0 + i * kChunk, y[0], y[1], y[2], y[3]);
+    st_shared_v4(p1 + i * kChunk, y[4], y[5], y[6], y[7]);
+  }
+}
+
+template <bool kFp4>
+__device__ __forceinline__ bool fine_tile(int tile) {
+  return !kFp4 && tile < kFineTiles;
+}
+
 // Walks the tiles of a CTA's range.
 struct Walk {
   int64_t row;
@@ -596,6 +637,8 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
     }
     mbar_init(&sm.rfull, 1);
     mbar_init(&sm.rempty, kLoadWarps);
+    mbar_init(&sm.lfull, kLoadWarps);
+    mbar_init(&sm.lempty, 1);
     mbar_init(&sm.qfull, kQWarps);
     mbar_init(&sm.qempty, 1);
     mbar_init(&sm.oempty, kSoftWarps);
@@ -622,28 +665,36 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
     // ------------------------------------------------ loaders
     const int lw = warp - kLoadWarp, tok = lw * 8 + (lane >> 2);
     const uint32_t mine = smem_u32(sm.raw) + tok * (kFp4 ? kRawFp4 : kRawFp8);
-    int tile = tile0, seg = 0;
+    // The remainders of a fine tile take the other K buffer between two tiles.
+    int tile = tile0, seg = 0, rests = 0;
+    bool was_fine = false;
     for (int g = 0; g < n; ++g) {
       const int b = g & 1;
       mbar_wait(&sm.rfull, g & 1, abort, &g_hcu_status);
       const uint32_t m0 = sm.mask[0], m1 = sm.mask[1];
-      const bool some = (m0 | m1) != 0;
+      const bool some = (m0 | m1) != 0, fine = fine_tile<kFp4>(tile);
       const bool on = (tok < 32 ? m0 >> tok : m1 >> (tok - 32)) & 1;
+      // The next gather writes the raw slots through the async proxy: without the proxy fence it overtook
+      // reads that were still under way (about one row of 2048 tokens x 64 heads in 500 came out wrong).
+      const auto release = [&] {
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.rempty);
+      };
       Conv conv;
       if (some) {
         Raw<kFp4> raw;
         read_raw<kFp4>(mine, lane & 3, raw);
-        // The next gather writes these bytes through the async proxy: without the proxy fence it overtook
-        // reads that were still under way (about one row of 2048 tokens x 64 heads in 500 came out wrong).
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.rempty);
+        if (!fine) release();
         convert<kFp4>(raw, lane & 3, conv);
       } else {
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.rempty);
       }
-      if (g >= 2) mbar_wait(&sm.empty[b], ((g >> 1) - 1) & 1, abort, &g_hcu_status);
+      if (was_fine)
+        mbar_wait(&sm.lempty, (rests - 1) & 1, abort, &g_hcu_status);
+      else if (g >= 2)
+        mbar_wait(&sm.empty[b], ((g >> 1) - 1) & 1, abort, &g_hcu_status);
       if (some) {
         store_tile(sm, b, lw, lane, on, conv);
         fence_async_shared();
@@ -655,6 +706,17 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.full[b]);
+      if (fine) {
+        if (g >= 1) mbar_wait(&sm.empty[b ^ 1], ((g - 1) >> 1) & 1, abort, &g_hcu_status);
+        if (some) {
+          store_rest(sm, b ^ 1, lw, lane, mine, conv.eb);
+          release();  // the fence is the remainders' too
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.lfull);
+        ++rests;
+      }
+      was_fine = fine;
       if (++tile == p.tiles) tile = 0;
     }
   } else if (warp == kGatherWarp) {
@@ -728,6 +790,7 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
       uint32_t s_none = 0;  // bit b: the tile in buffer b holds no token
       uint32_t acc = 0;     // the segment's O holds something
       bool q_ok = false;    // the segment's Q has been waited for
+      int rests = 0;        // fine tiles so far
       uint64_t t0 = 0;
       int idle = 0;
       while (o < n) {
@@ -735,7 +798,8 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
         if (s < n && s < o + 2) {
           const int b = s & 1;
           if (!q_ok) q_ok = mbar_test(&sm.qfull, s_seg & 1);
-          if (q_ok && mbar_test(&sm.full[b], (s >> 1) & 1)) {
+          const bool fine = fine_tile<kFp4>(s_tile);
+          if (q_ok && mbar_test(&sm.full[b], (s >> 1) & 1) && (!fine || mbar_test(&sm.lfull, rests & 1))) {
             moved = true;
             tc_fence_after();
             s_none &= ~(1u << b);
@@ -747,9 +811,24 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
                 mma_f16(tmem + kTmemS + 64 * b, qd + ((c * kQChunk + off) >> 4), kd + ((c * kChunk + off) >> 4), id_s,
                         k > 0 ? 1u : 0u);
               }
+              if (fine) {
+                const uint64_t rd = sw128_kmajor_desc(smem_u32(sm.k[b ^ 1]));
+#pragma unroll 1
+                for (int c = 0; c < kLatentDim / 64; ++c)
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    mma_f16(tmem + kTmemS + 64 * b, qd + ((c * kQChunk + 32 * j) >> 4), rd + ((c * kChunk + 32 * j) >> 4),
+                            id_s, 1u);
+                tc_commit(&sm.lempty);
+                ++rests;
+              }
               tc_commit(&sm.sfull[b]);
             } else {
               s_none |= 1u << b;
+              if (fine) {
+                mbar_arrive(&sm.lempty);
+                ++rests;
+              }
               mbar_arrive(&sm.sfull[b]);
             }
             ++s;
