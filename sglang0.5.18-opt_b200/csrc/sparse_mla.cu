@@ -15,41 +15,41 @@
 //     registers, which frees the raw buffer, and store them as the tile's K once a K buffer is free: 9
 //     chunks of [48 tokens][64 values], rows of 128 bytes, 128-byte swizzle.  A chunk is a K-major
 //     operand for q k^T and, read the other way, an MN-major one for v^T, so the latent is stored once;
-//   * 4 warps bring each segment's Q in and convert it in place (f16, K-major);
+//   * 4 warps bring each segment's Q in as f16: two chunks to TMEM, seven to shared memory;
 //   * the MMA thread issues S = Q K^T (M = 64 heads, N = 48 tokens, K = 576) and, up to two tiles
 //     behind, O^T += V^T P^T (M = 128 latent values x 4, N = heads, K = 48 tokens): with the latent as M
 //     the second product runs at the full rate, and O^T takes 4 x 64 TMEM columns;
 //   * 4 softmax warps (16 heads each) read S, keep the running maximum and sum in fp32 and write P
 //     in f16 over the tile's rope chunk, which S no longer needs.  O^T is rescaled only when a
 //     maximum has risen by more than 2^kLazy.
-// 48 tokens: Q (74 KB), two K tiles (55 KB each) and the raw slots (34 KB) fill the 227 KB.
+// 48 tokens: Q (57 KB), two K tiles (55 KB each), three more P (18 KB, below) and the raw slots (34 KB)
+// fill the 227 KB.
 //
 // Number format.  f16 operands hold 11 bits where bf16 holds 8, and an fp8 or e2m1 value is exact in
 // f16; its range is met by powers of two taken out per token and per query row:
-//   * token t: 2^E, E from its largest scale; latent codes are multiplied by scale * 2^-E (rounded to
-//     f16, exact for the 4-bit slot's power of two) and the rope by 2^-E 2^-10; E is raised where the
-//     rope would leave f16's range (latents 2^-35 below the rope);
+//   * token t: 2^E, E from its largest scale; latent codes are multiplied by scale * 2^-E and the rope by
+//     2^-E 2^-10; E is raised where the rope would leave f16's range (latents 2^-35 below the rope);
 //   * query row: 2^e, its largest element just below 2^4 (latent part) or 2^14 (rope part, which
 //     takes the 2^10 back), so elements down to 2^-18 of the largest keep all their bits.
-// What is rounded, then, is an fp8 value times its scale's mantissa, once in the factor and once in the
-// product; 4-bit values are exact.  Over many tokens the scores' errors of 5e-4 average out (lse of 2048
-// tokens is 4e-6 of itself off, out less than its own bf16 rounding), over few they do not (33 tokens:
-// 5e-5).  A row of few tokens has them in its first tiles, so the first two tiles of a job multiply Q with
-// what the rounding left out as well: lse is off by 7e-7 of itself up to 96 tokens and 1e-5 at most
-// beyond (200 tokens).
+// Nothing of a 4-bit slot is rounded: its token scale is a power of two, code * group scale six bits.  An
+// fp8 group's scale has 24, and rounded products put lse of 33 tokens 5e-5 of itself off.  So scales are
+// rounded to 7 bits, whose products with a value's 4 are exact, and what a scale is of its rounding,
+// r = 1 +- 2^-8, is put in where a group's sums are: S has a part per 128-value group, s = sum_g r_g S_g in
+// fp32, and block g of O^T takes P r_g, a P of its own.  The rope joins S_3, divided by r_3: the one
+// operand that is rounded (2^-12 each).  lse of 33 tokens is 8e-6 of itself off, of 2048 tokens 8e-7.
 //
 // S * 2^(E + e) is the score; P carries 2^E of its token in its exponent (w = s + E, whose maximum is
 // the running one), so O needs no correction, and the sum takes 2^-E back per token.
 //
 // Bound.  A 48-token tile needs 1370 cycles of the tensor pipe (940 for S, whose M of 64 fills half of
 // it, 430 for O) and about 2500 of the shared-memory port at 128 B per cycle (34 KB of raw slots in and
-// out, 55 KB of K in, 126 KB of Q and K operands for S, 72 KB of V and P for O); it takes 3300.  What is
-// left is the chain of a tile through its warps (copy 2900, convert 650, store 1000, S 940, softmax
-// 1250, O 430 cycles), with two K tiles and one of raw slots to overlap it.  Both were traded: Q partly
-// in TMEM makes room for a third K tile (7 % slower) or a second raw buffer (11 %), copies of 16 bytes from
-// the loader warps replace the raw ring (14 to 19 %).  2048 rows x 64 heads x 2048 fp8 tokens (584 GFLOP)
-// take 1.085 ms, 538 TFLOP/s; 128 rows 91 us; one row 27 us; 192 rows of 4-bit slots 138 us (no
-// remainders, a conversion 500 cycles longer).  L2 flushed before each call.
+// out, 55 KB of K and 24 KB of P in, 110 KB of Q and K operands for S, 72 KB of V and P for O); it takes
+// 4100 (fp8).  What is left is the chain of a tile through its warps (copy 2900, convert 650, store 1000,
+// S 940, softmax 1250 with one P, O 430 cycles), with two K tiles and one of raw slots to overlap it.  Both
+// were traded, with one P: a third K tile took 7 % longer, a second raw buffer 11 %, copies of 16 bytes from
+// the loader warps in place of the raw ring 14 to 19 %.  2048 rows x 64 heads x 2048 fp8 tokens (584 GFLOP)
+// take 1.28 ms, 456 TFLOP/s (1.015 with rounded scales, one S and one P); 128 rows 103 us; one row 26 us;
+// 192 rows of 4-bit slots 138 us.  L2 flushed before each call.
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 
@@ -70,6 +70,8 @@ constexpr int kChunks = kQkDim / 64;
 constexpr int kQChunk = kHg * 128;     // [64 heads][64 f16]
 constexpr int kChunk = kTile * 128;    // [48 tokens][64 f16]
 constexpr int kTileBytes = kChunks * kChunk;
+constexpr int kPBytes = kTile * kHg * 2;
+constexpr int kQTmem = 2;              // chunks of Q in TMEM, the others in shared memory
 constexpr int kRawFp8 = 704, kRawFp4 = 480;  // a slot's row in the raw buffer (see Raw), the slot padded with zeros
 constexpr int kSoftWarps = 4;
 constexpr int kMmaWarp = kSoftWarps;
@@ -81,7 +83,8 @@ constexpr int kLoadWarps = kTile / 8;
 constexpr int kAtThreads = (kLoadWarp + kLoadWarps) * 32;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kTmemO = 0;    // 4 blocks of 128 latent values x 64 heads
-constexpr uint32_t kTmemS = 256;  // 2 score buffers of 48 columns, 64 apart
+constexpr uint32_t kTmemS = 256;  // fp8: 4 score parts of 48 columns; 4-bit: 2 score buffers, 64 apart
+constexpr uint32_t kTmemQ = 448;  // 32 columns a chunk
 // P is 2^(w - m + kBias), m the row's maximum when it was last taken: the largest weight is 2^8 then,
 // 2^15 while the maximum has grown by the tolerated 2^kLazy (scores of a row with a spread of 2.2 in
 // base 2 hardly ever rise by 7 over their first 48's maximum), and weights down to 2^-22 of the
@@ -89,17 +92,15 @@ constexpr uint32_t kTmemS = 256;  // 2 score buffers of 48 columns, 64 apart
 constexpr float kLazy = 7.f;
 constexpr float kBias = 8.f;
 constexpr int kRopeShift = 10;
-// Tiles at a job's start whose fp8 values are multiplied with their rounding's remainder too (see the
-// number format): 2048 rows x 64 heads x 2048 tokens take 1.085 ms with two of them, 1.015 without any.
-// One leaves lse of 130 to 200 tokens at the edge of 2e-5 of itself.
-constexpr int kFineTiles = 2;
 constexpr int kPartFloats = kHg * kLatentDim + kHg;
 
 struct __align__(1024) AtSmem {
-  uint8_t q[kChunks * kQChunk];
+  uint8_t q[(kChunks - kQTmem) * kQChunk];
   uint8_t k[2][kTileBytes];
+  uint8_t p[3][kPBytes];  // fp8: P of groups 1 to 3 (of group 0, as the only P of 4-bit slots: the tile's rope chunk)
   __align__(128) uint8_t raw[kTile * kRawFp8];  // slots of the tile to be converted next, as they are in the cache
   __align__(16) uint8_t stage[kSoftWarps][1024];  // output rows on their way out
+  float4 tok_r[2][kTile];   // fp8: what each group's scale is of its 7-bit rounding
   float tok_e[2][kTile];    // E of each token (-inf: no token)
   float tok_up[2][kTile];   // 2^E (0: no token)
   float tok_dn[2][kTile];   // 2^-E (0: no token)
@@ -108,7 +109,7 @@ struct __align__(1024) AtSmem {
   uint32_t mask[2];         // candidates in raw that are tokens
   int empty_tile[2];        // the tile in buffer b holds no token
   uint64_t full[2], empty[2], sfull[2], pready[2];
-  uint64_t rfull, rempty, lfull, lempty, qfull, qempty, oempty, done;
+  uint64_t rfull, rempty, sempty, qfull, qempty, oempty, done;
   uint32_t tmem;
   int abort;
 };
@@ -148,6 +149,17 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// The same with A in TMEM.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -219,6 +231,40 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_st_16x256_x8(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x8.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+
+// The four score parts' columns of 16 tokens: r[g] as tmem_ld_scores' first 8 of part g.
+__device__ __forceinline__ void tmem_ld_parts(uint32_t taddr, uint32_t (&r)[4][8]) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[g][0]), "=r"(r[g][1]), "=r"(r[g][2]), "=r"(r[g][3]), "=r"(r[g][4]), "=r"(r[g][5]),
+                   "=r"(r[g][6]), "=r"(r[g][7])
+                 : "r"(taddr + kTile * g)
+                 : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0][0]), "+r"(r[0][1]), "+r"(r[0][2]), "+r"(r[0][3]), "+r"(r[0][4]), "+r"(r[0][5]),
+                 "+r"(r[0][6]), "+r"(r[0][7]), "+r"(r[1][0]), "+r"(r[1][1]), "+r"(r[1][2]), "+r"(r[1][3]),
+                 "+r"(r[1][4]), "+r"(r[1][5]), "+r"(r[1][6]), "+r"(r[1][7])
+               :
+               : "memory");
+  asm volatile(""
+               : "+r"(r[2][0]), "+r"(r[2][1]), "+r"(r[2][2]), "+r"(r[2][3]), "+r"(r[2][4]), "+r"(r[2][5]),
+                 "+r"(r[2][6]), "+r"(r[2][7]), "+r"(r[3][0]), "+r"(r[3][1]), "+r"(r[3][2]), "+r"(r[3][3]),
+                 "+r"(r[3][4]), "+r"(r[3][5]), "+r"(r[3][6]), "+r"(r[3][7])
+               :
+               : "memory");
+}
+
 __device__ __forceinline__ void stmatrix_x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
                "r"(d)
@@ -284,6 +330,11 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
   return ok != 0;
+}
+
+__device__ __forceinline__ uint32_t pack2(float2 v) {
+  const __half2 h = __floats2half2_rn(v.x, v.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // OR of a predicate over the softmax warps.
@@ -458,32 +509,51 @@ __device__ __forceinline__ int exponent2(__nv_bfloat162 m) {
 
 __device__ __forceinline__ float exp2_of(int biased) { return __uint_as_float(static_cast<uint32_t>(biased) << 23); }
 
-// Heads 8 hp .. 8 hp + 7 of a job, four lanes each: 18 pieces of 16 bytes a lane straight to their
-// places in the Q buffer as bf16 (copy_q), converted in place once they are there (convert_q).
+// Q of a job, 16 heads a warp: lane l owns a quarter (sub = l % 4) of heads l / 4 and l / 4 + 8 of them.
+// The first two chunks go to TMEM as fragments of 8 columns (16 values), values 16 j + 4 sub .. + 3 of both
+// heads for step j, from registers (fetch_q); the others straight to their places in the Q buffer as
+// bf16, 14 pieces of 16 bytes a head and lane (copy_q), converted in place once they are there.
 // cq[h] is the head's factor from the product to the score in base 2.
-__device__ __forceinline__ uint32_t q_piece(uint32_t base, int hp, int hr, int u) {
-  return base + hp * 1024 + hr * 128 + (u >> 3) * kQChunk + (((u & 7) ^ hr) << 4);
+constexpr int kQPieces = 2 * (kChunks - kQTmem);  // a lane's, per head
+
+__device__ __forceinline__ const uint16_t* q_head(const AttnArgs& p, int64_t row, int h) {
+  // a head past the last reads head 0: rows of S and columns of O are independent, and its are not stored
+  return p.q + row * p.q_row + (h < p.heads ? h * p.q_head : 0);
 }
 
-__device__ __forceinline__ void copy_q(const AttnArgs& p, uint32_t q, int64_t row, int h0, int hp, int lane) {
-  const int hr = lane >> 2, sub = lane & 3, h = h0 + hp * 8 + hr;
-  // a head past the last reads head 0: rows of S and columns of O are independent, and its are not stored
-  const uint4* src = reinterpret_cast<const uint4*>(p.q + row * p.q_row + (h < p.heads ? h * p.q_head : 0));
+__device__ __forceinline__ uint32_t q_piece(uint32_t base, int h, int u) {
+  return base + h * 128 + (u >> 3) * kQChunk + (((u & 7) ^ (h & 7)) << 4);
+}
+
+__device__ __forceinline__ uint2 ldg_v2(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ void fetch_q(const uint16_t* q, int sub, uint2 (&v)[8]) {
 #pragma unroll
-  for (int i = 0; i < 18; ++i)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(q_piece(q, hp, hr, sub + 4 * i)),
-                 "l"(src + sub + 4 * i)
+  for (int j = 0; j < 8; ++j) v[j] = ldg_v2(q + 16 * j + 4 * sub);
+}
+
+__device__ __forceinline__ void copy_q(const uint16_t* q, uint32_t dst, int h, int sub) {
+#pragma unroll
+  for (int i = 0; i < kQPieces; ++i)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(q_piece(dst, h, sub + 4 * i)),
+                 "l"(q + 64 * kQTmem + 8 * (sub + 4 * i))
                  : "memory");
 }
 
-__device__ __forceinline__ void convert_q(const AttnArgs& p, uint32_t q, float* cq, int hp, int lane) {
-  const int hr = lane >> 2, sub = lane & 3;
-  uint4 v[18];
+// Returns the factor of the head's latent part.
+__device__ __forceinline__ float convert_q(const AttnArgs& p, uint32_t q, float* cq, int h, int sub, const uint2 (&t)[8]) {
+  uint4 v[kQPieces];
 #pragma unroll
-  for (int i = 0; i < 18; ++i) v[i] = ld_shared_v4(q_piece(q, hp, hr, sub + 4 * i));
+  for (int i = 0; i < kQPieces; ++i) v[i] = ld_shared_v4(q_piece(q, h, sub + 4 * i));
   __nv_bfloat162 am = amax8(v[0]);
 #pragma unroll
-  for (int i = 1; i < 18; ++i) am = __hmax2(am, amax8(v[i]));
+  for (int i = 1; i < kQPieces; ++i) am = __hmax2(am, amax8(v[i]));
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) am = __hmax2(am, amax8(make_uint4(t[j].x, t[j].y, t[j + 1].x, t[j + 1].y)));
   int eb = exponent2(am);
   eb = max(eb, __shfl_xor_sync(0xffffffffu, eb, 1));
   eb = max(eb, __shfl_xor_sync(0xffffffffu, eb, 2));
@@ -491,12 +561,13 @@ __device__ __forceinline__ void convert_q(const AttnArgs& p, uint32_t q, float* 
   const float f_lat = exp2_of(254 - eb + 3);    // the largest into [2^3, 2^4)
   const float f_rope = exp2_of(254 - eb + 13);  // 2^10 more
 #pragma unroll
-  for (int i = 0; i < 18; ++i) {
-    const float f = i < 16 ? f_lat : f_rope;
-    st_shared_v4(q_piece(q, hp, hr, sub + 4 * i), bf2_to_h2(v[i].x, f), bf2_to_h2(v[i].y, f), bf2_to_h2(v[i].z, f),
+  for (int i = 0; i < kQPieces; ++i) {
+    const float f = i < kQPieces - 2 ? f_lat : f_rope;
+    st_shared_v4(q_piece(q, h, sub + 4 * i), bf2_to_h2(v[i].x, f), bf2_to_h2(v[i].y, f), bf2_to_h2(v[i].z, f),
                  bf2_to_h2(v[i].w, f));
   }
-  if (sub == 0) cq[hp * 8 + hr] = p.sm_scale * 1.4426950408889634f * exp2_of(eb - 3);
+  if (sub == 0) cq[h] = p.sm_scale * 1.4426950408889634f * exp2_of(eb - 3);
+  return f_lat;
 }
 
 // A lane's converted share of a tile, held in registers until the tile's buffer is free.
@@ -504,6 +575,7 @@ struct Conv {
   uint32_t y[8][8];  // latent elements 64 i + 16 sub .. + 15, two f16 a word
   uint32_t r[8];     // rope
   int eb;            // biased exponent taken out of the token
+  float rest;        // fp8: group sub's scale over its rounding
 };
 
 template <bool kFp4>
@@ -516,7 +588,23 @@ __device__ __forceinline__ void convert(const Raw<kFp4>& r, int sub, Conv& c) {
     smax = max(max(smax, r.sc.y & 0x7fffffffu), max(r.sc.z & 0x7fffffffu, r.sc.w & 0x7fffffffu));
   c.eb = min(max(max(static_cast<int>(smax >> 23), re - 13 - kRopeShift), 27), 247);
   const float dn = exp2_of(254 - c.eb);
-  const float fr = dn * (1.f / (1 << kRopeShift));
+  float fr = dn * (1.f / (1 << kRopeShift));
+  __half2 scale[4];
+  if constexpr (!kFp4) {
+    // scales to 7 bits, so that their products with an fp8 value's 4 are exact in f16's 11
+    const uint32_t w[4] = {r.sc.x, r.sc.y, r.sc.z, r.sc.w};
+    float f = 0.f, h = 0.f;  // group sub's scale and its rounding
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float x = __uint_as_float(w[g]) * dn;
+      scale[g] = __float2half2_rn(__uint_as_float((__float_as_uint(x) + 0x10000u) & 0xfffe0000u));
+      f = g == sub ? x : f;
+      h = g == sub ? __low2float(scale[g]) : h;
+    }
+    c.rest = h != 0.f ? __fdividef(f, h) : 1.f;  // h is 0 where the group is 2^-25 of the token's largest
+    // the rope shares group 3's part of the score
+    fr = __fdividef(fr, __shfl_sync(0xffffffffu, c.rest, (threadIdx.x & 31) | 3));
+  }
   const uint32_t rw[8] = {r.rope[0].x, r.rope[0].y, r.rope[0].z, r.rope[0].w,
                           r.rope[1].x, r.rope[1].y, r.rope[1].z, r.rope[1].w};
 #pragma unroll
@@ -534,8 +622,7 @@ __device__ __forceinline__ void convert(const Raw<kFp4>& r, int sub, Conv& c) {
         c.y[i][4 + k] = h2_bits(__hmul2(e2m1x2_to_half2((r.y[i].y >> (8 * k)) & 0xff), s));
       }
     } else {
-      const uint32_t w = i < 2 ? r.sc.x : i < 4 ? r.sc.y : i < 6 ? r.sc.z : r.sc.w;
-      const __half2 s = __float2half2_rn(__uint_as_float(w) * dn);
+      const __half2 s = scale[i >> 1];
       const uint32_t x[4] = {r.x[i].x, r.x[i].y, r.x[i].z, r.x[i].w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -547,8 +634,10 @@ __device__ __forceinline__ void convert(const Raw<kFp4>& r, int sub, Conv& c) {
 }
 
 // Stores the warp's 8 tokens as rows 8 lw .. 8 lw + 7 of tile buffer b; on: the lane's token exists.
+template <bool kFp4>
 __device__ __forceinline__ void store_tile(AtSmem& sm, int b, int lw, int lane, bool on, const Conv& c) {
   const int tok = lane >> 2, sub = lane & 3;
+  if constexpr (!kFp4) reinterpret_cast<float*>(&sm.tok_r[b][lw * 8 + tok])[sub] = c.rest;
   if (sub == 0) {
     const int t = lw * 8 + tok;
     sm.tok_e[b][t] = on ? static_cast<float>(c.eb - 127) : -INFINITY;
@@ -564,36 +653,6 @@ __device__ __forceinline__ void store_tile(AtSmem& sm, int b, int lw, int lane, 
   });
   st_shared_v4<8 * kChunk>(p0, c.r[0], c.r[1], c.r[2], c.r[3]);
   st_shared_v4<8 * kChunk>(p1, c.r[4], c.r[5], c.r[6], c.r[7]);
-}
-
-// The remainders of the warp's 8 tokens, fp8 value * scale - what store_tile stored, as rows of buffer b.
-// Unscaled: below f16's normal range they lose bits that are 2^-24 of a latent of 1, where the largest
-// is 2^8 to 2^10.
-__device__ __forceinline__ void store_rest(AtSmem& sm, int b, int lw, int lane, uint32_t row, int eb) {
-  const int tok = lane >> 2, sub = lane & 3;
-  const uint32_t p0 = smem_u32(sm.k[b]) + lw * 1024 + tok * 128 + (((2 * sub) ^ tok) << 4), p1 = p0 ^ 16u;
-  const float dn = exp2_of(254 - eb);
-#pragma unroll 2
-  for (int i = 0; i < 8; ++i) {
-    const uint4 x = ld_shared_v4(row + 64 * i + 16 * sub);
-    const float f = __uint_as_float(ld_shared_u32(row + kFp8Scales + 4 * (i >> 1))) * dn;
-    const __half2 s = __float2half2_rn(f);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    uint32_t y[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const __half2 c = e4m3x2_to_half2(w[k >> 1] >> (16 * (k & 1)) & 0xffffu);
-      const float2 v = __half22float2(c), hi = __half22float2(__hmul2(c, s));
-      y[k] = h2_bits(__floats2half2_rn(fmaf(v.x, f, -hi.x), fmaf(v.y, f, -hi.y)));
-    }
-    st_shared_v4(p0 + i * kChunk, y[0], y[1], y[2], y[3]);
-    st_shared_v4(p1 + i * kChunk, y[4], y[5], y[6], y[7]);
-  }
-}
-
-template <bool kFp4>
-__device__ __forceinline__ bool fine_tile(int tile) {
-  return !kFp4 && tile < kFineTiles;
 }
 
 // Walks the tiles of a CTA's range.
@@ -637,8 +696,7 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
     }
     mbar_init(&sm.rfull, 1);
     mbar_init(&sm.rempty, kLoadWarps);
-    mbar_init(&sm.lfull, kLoadWarps);
-    mbar_init(&sm.lempty, 1);
+    mbar_init(&sm.sempty, kSoftWarps);
     mbar_init(&sm.qfull, kQWarps);
     mbar_init(&sm.qempty, 1);
     mbar_init(&sm.oempty, kSoftWarps);
@@ -665,38 +723,30 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
     // ------------------------------------------------ loaders
     const int lw = warp - kLoadWarp, tok = lw * 8 + (lane >> 2);
     const uint32_t mine = smem_u32(sm.raw) + tok * (kFp4 ? kRawFp4 : kRawFp8);
-    // The remainders of a fine tile take the other K buffer between two tiles.
-    int tile = tile0, seg = 0, rests = 0;
-    bool was_fine = false;
+    int tile = tile0, seg = 0;
     for (int g = 0; g < n; ++g) {
       const int b = g & 1;
       mbar_wait(&sm.rfull, g & 1, abort, &g_hcu_status);
       const uint32_t m0 = sm.mask[0], m1 = sm.mask[1];
-      const bool some = (m0 | m1) != 0, fine = fine_tile<kFp4>(tile);
+      const bool some = (m0 | m1) != 0;
       const bool on = (tok < 32 ? m0 >> tok : m1 >> (tok - 32)) & 1;
-      // The next gather writes the raw slots through the async proxy: without the proxy fence it overtook
-      // reads that were still under way (about one row of 2048 tokens x 64 heads in 500 came out wrong).
-      const auto release = [&] {
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.rempty);
-      };
       Conv conv;
       if (some) {
         Raw<kFp4> raw;
         read_raw<kFp4>(mine, lane & 3, raw);
-        if (!fine) release();
+        // The next gather writes these bytes through the async proxy: without the proxy fence it overtook
+        // reads that were still under way (about one row of 2048 tokens x 64 heads in 500 came out wrong).
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.rempty);
         convert<kFp4>(raw, lane & 3, conv);
       } else {
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.rempty);
       }
-      if (was_fine)
-        mbar_wait(&sm.lempty, (rests - 1) & 1, abort, &g_hcu_status);
-      else if (g >= 2)
-        mbar_wait(&sm.empty[b], ((g >> 1) - 1) & 1, abort, &g_hcu_status);
+      if (g >= 2) mbar_wait(&sm.empty[b], ((g >> 1) - 1) & 1, abort, &g_hcu_status);
       if (some) {
-        store_tile(sm, b, lw, lane, on, conv);
+        store_tile<kFp4>(sm, b, lw, lane, on, conv);
         fence_async_shared();
       }
       if (lw == 0) {
@@ -706,17 +756,6 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.full[b]);
-      if (fine) {
-        if (g >= 1) mbar_wait(&sm.empty[b ^ 1], ((g - 1) >> 1) & 1, abort, &g_hcu_status);
-        if (some) {
-          store_rest(sm, b ^ 1, lw, lane, mine, conv.eb);
-          release();  // the fence is the remainders' too
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.lfull);
-        ++rests;
-      }
-      was_fine = fine;
       if (++tile == p.tiles) tile = 0;
     }
   } else if (warp == kGatherWarp) {
@@ -790,7 +829,6 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
       uint32_t s_none = 0;  // bit b: the tile in buffer b holds no token
       uint32_t acc = 0;     // the segment's O holds something
       bool q_ok = false;    // the segment's Q has been waited for
-      int rests = 0;        // fine tiles so far
       uint64_t t0 = 0;
       int idle = 0;
       while (o < n) {
@@ -798,8 +836,8 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
         if (s < n && s < o + 2) {
           const int b = s & 1;
           if (!q_ok) q_ok = mbar_test(&sm.qfull, s_seg & 1);
-          const bool fine = fine_tile<kFp4>(s_tile);
-          if (q_ok && mbar_test(&sm.full[b], (s >> 1) & 1) && (!fine || mbar_test(&sm.lfull, rests & 1))) {
+          // the fp8 score parts have one buffer, which the softmax warps empty into registers
+          if (q_ok && mbar_test(&sm.full[b], (s >> 1) & 1) && (kFp4 || s == 0 || mbar_test(&sm.sempty, (s - 1) & 1))) {
             moved = true;
             tc_fence_after();
             s_none &= ~(1u << b);
@@ -808,27 +846,17 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
 #pragma unroll
               for (int k = 0; k < kQkDim / 16; ++k) {
                 const uint32_t c = k >> 2, off = (k & 3) * 32;
-                mma_f16(tmem + kTmemS + 64 * b, qd + ((c * kQChunk + off) >> 4), kd + ((c * kChunk + off) >> 4), id_s,
-                        k > 0 ? 1u : 0u);
-              }
-              if (fine) {
-                const uint64_t rd = sw128_kmajor_desc(smem_u32(sm.k[b ^ 1]));
-#pragma unroll 1
-                for (int c = 0; c < kLatentDim / 64; ++c)
-#pragma unroll
-                  for (int j = 0; j < 4; ++j)
-                    mma_f16(tmem + kTmemS + 64 * b, qd + ((c * kQChunk + 32 * j) >> 4), rd + ((c * kChunk + 32 * j) >> 4),
-                            id_s, 1u);
-                tc_commit(&sm.lempty);
-                ++rests;
+                const uint32_t g = c >> 1 < 3 ? c >> 1 : 3;  // 128 values; the rope is the last one's
+                const uint32_t d = tmem + kTmemS + (kFp4 ? 64 * b : kTile * g);
+                const uint32_t add = (kFp4 ? k == 0 : k % 8 == 0 && c < 8) ? 0u : 1u;
+                if (c < kQTmem)
+                  mma_f16_ts(d, tmem + kTmemQ + 8 * k, kd + ((c * kChunk + off) >> 4), id_s, add);
+                else
+                  mma_f16(d, qd + (((c - kQTmem) * kQChunk + off) >> 4), kd + ((c * kChunk + off) >> 4), id_s, add);
               }
               tc_commit(&sm.sfull[b]);
             } else {
               s_none |= 1u << b;
-              if (fine) {
-                mbar_arrive(&sm.lempty);
-                ++rests;
-              }
               mbar_arrive(&sm.sfull[b]);
             }
             ++s;
@@ -854,12 +882,13 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
               tc_fence_after();
               const uint32_t id_o = idesc_f16(128, (min(kHg, p.heads - o_hg * kHg) + 15) & ~15, true);
               const uint64_t v = sw128_mnmajor_desc(smem_u32(sm.k[b]));
-              const uint64_t pd = sw32_kmajor_desc(smem_u32(sm.k[b]) + 8 * kChunk);
+              const uint64_t pd = sw32_kmajor_desc(smem_u32(sm.k[b]) + 8 * kChunk), px = sw32_kmajor_desc(smem_u32(sm.p[0]));
 #pragma unroll
               for (int ks = 0; ks < kTile / 16; ++ks)
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
-                  mma_f16(tmem + kTmemO + 64 * d, v + ((2 * d * kChunk + ks * 2048) >> 4), pd + ((ks * 2048) >> 4), id_o,
+                  mma_f16(tmem + kTmemO + 64 * d, v + ((2 * d * kChunk + ks * 2048) >> 4),
+                          (kFp4 || d == 0 ? pd : px + (((d - 1) * kPBytes) >> 4)) + ((ks * 2048) >> 4), id_o,
                           ks > 0 ? 1u : acc);
               acc = 1;
               tc_commit(&sm.empty[b]);
@@ -890,17 +919,33 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
     // ------------------------------------------------ queries
     // Q is single-buffered: the next segment's rows are brought into L2 while this one's are in use.
     // Four cq buffers: when a segment's Q is released, its second predecessor's first tile is done with.
-    const int qw = warp - kQWarp;
+    const int qw = warp - kQWarp, quad = warp & 3, sub = lane & 3, h0 = 16 * quad + (lane >> 2);
     Walk at(p, job0, 0);
     const int segs = (tile0 + n + p.tiles - 1) / p.tiles;
     for (int seg = 0; seg < segs; ++seg) {
+      uint2 v[2][8];
+      float f[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) fetch_q(q_head(p, at.row, at.hg * kHg + h0 + 8 * i), sub, v[i]);
       if (seg > 0) mbar_wait(&sm.qempty, (seg - 1) & 1, abort, &g_hcu_status);
+      tc_fence_after();
       const uint32_t q = smem_u32(sm.q);
-#pragma unroll 1
-      for (int hp = qw; hp < kHg / 8; hp += kQWarps) copy_q(p, q, at.row, at.hg * kHg, hp, lane);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) copy_q(q_head(p, at.row, at.hg * kHg + h0 + 8 * i), q, h0 + 8 * i, sub);
       asm volatile("cp.async.wait_all;" ::: "memory");  // each lane converts what it copied
-#pragma unroll 1
-      for (int hp = qw; hp < kHg / 8; hp += kQWarps) convert_q(p, q, sm.cq[seg & 3], hp, lane);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) f[i] = convert_q(p, q, sm.cq[seg & 3], h0 + 8 * i, sub, v[i]);
+      uint32_t r[32];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          r[4 * j + 2 * i] = bf2_to_h2(v[i][j].x, f[i]);
+          r[4 * j + 2 * i + 1] = bf2_to_h2(v[i][j].y, f[i]);
+        }
+      tmem_st_16x256_x8(tmem + kTmemQ + (static_cast<uint32_t>(quad * 32) << 16), r);
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc_fence_before();
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.qfull);
@@ -932,12 +977,11 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
         cq1 = sm.cq[seg & 3][r1];
         started = false;
       }
-      float2 up[6], e[6], dn[6];  // of the thread's tokens, read while S is computed
+      float2 up[6], e[6];  // of the thread's tokens, read while S is computed
 #pragma unroll
       for (int i = 0; i < 6; ++i) {
         up[i] = *reinterpret_cast<const float2*>(&sm.tok_up[b][8 * i + cl]);
         e[i] = *reinterpret_cast<const float2*>(&sm.tok_e[b][8 * i + cl]);
-        dn[i] = *reinterpret_cast<const float2*>(&sm.tok_dn[b][8 * i + cl]);
       }
       const bool none = sm.empty_tile[b];
       mbar_wait(&sm.sfull[b], (g >> 1) & 1, abort, &g_hcu_status);
@@ -947,23 +991,49 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
       float mx0 = -INFINITY, mx1 = -INFINITY;
       if (!none) {
         tc_fence_after();
-        uint32_t s[24];
-        tmem_ld_scores(tmem + kTmemS + 64 * b + quad, s);
         const float2 c0 = make_float2(cq0, cq0), c1 = make_float2(cq1, cq1);
-#pragma unroll
-        for (int i = 0; i < 6; ++i) {
-          const float2 a = make_float2(__uint_as_float(s[4 * i]), __uint_as_float(s[4 * i + 1]));
-          const float2 d = make_float2(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3]));
+        const auto score = [&](int i, float2 a, float2 d) {
           w[2 * i] = __ffma2_rn(__fmul2_rn(a, up[i]), c0, e[i]);
           w[2 * i + 1] = __ffma2_rn(__fmul2_rn(d, up[i]), c1, e[i]);
           mx0 = fmaxf(mx0, fmaxf(w[2 * i].x, w[2 * i].y));
           mx1 = fmaxf(mx1, fmaxf(w[2 * i + 1].x, w[2 * i + 1].y));
+        };
+        if constexpr (kFp4) {
+          uint32_t s[24];
+          tmem_ld_scores(tmem + kTmemS + 64 * b + quad, s);
+#pragma unroll
+          for (int i = 0; i < 6; ++i)
+            score(i, make_float2(__uint_as_float(s[4 * i]), __uint_as_float(s[4 * i + 1])),
+                  make_float2(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3])));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 3; ++j) {
+            uint32_t s[4][8];
+            tmem_ld_parts(tmem + kTmemS + 16 * j + quad, s);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float4 x = sm.tok_r[b][16 * j + 8 * k + cl], y = sm.tok_r[b][16 * j + 8 * k + cl + 1];
+              const float2 r[4] = {make_float2(x.x, y.x), make_float2(x.y, y.y), make_float2(x.z, y.z), make_float2(x.w, y.w)};
+              float2 a = make_float2(0.f, 0.f), d = a;
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                a = __ffma2_rn(make_float2(__uint_as_float(s[g][4 * k]), __uint_as_float(s[g][4 * k + 1])), r[g], a);
+                d = __ffma2_rn(make_float2(__uint_as_float(s[g][4 * k + 2]), __uint_as_float(s[g][4 * k + 3])), r[g], d);
+              }
+              score(2 * j + k, a, d);
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.sempty);
         }
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) {
           mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
           mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
         }
+      } else if (!kFp4 && lane == 0) {
+        mbar_arrive(&sm.sempty);
       }
       if (soft_any(mx0 > m0 + kLazy || mx1 > m1 + kLazy)) {  // m = -inf: any finite maximum
         const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
@@ -1004,22 +1074,39 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
         // P: for every 16 tokens [64 heads][16 tokens], rows of 32 bytes with the 32-byte swizzle
         const int ph = 16 * warp + 8 * ((lane >> 3) & 1) + (lane & 7);
         const uint32_t pdst = smem_u32(sm.k[b]) + 8 * kChunk + st_piece(ph, lane >> 4);
+        const uint32_t pxdst = smem_u32(sm.p[0]) + st_piece(ph, lane >> 4);
+        // groups 1 to 3 have one buffer: the last tile's product has read it (the one before that came before
+        // this tile's scores)
+        if (!kFp4 && g > 0) mbar_wait(&sm.empty[(g - 1) & 1], ((g - 1) >> 1) & 1, abort, &g_hcu_status);
         const float2 n0 = make_float2(-b0, -b0), n1 = make_float2(-b1, -b1);
         float2 z0 = make_float2(l0, 0.f), z1 = make_float2(l1, 0.f);
 #pragma unroll
         for (int i = 0; i < 6; i += 2) {
-          uint32_t h[4];
+          float2 p0[2], p1[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const float2 x0 = __fadd2_rn(w[2 * (i + k)], n0), x1 = __fadd2_rn(w[2 * (i + k) + 1], n1);
-            const float2 p0 = make_float2(ex2(x0.x), ex2(x0.y)), p1 = make_float2(ex2(x1.x), ex2(x1.y));
-            z0 = __ffma2_rn(p0, dn[i + k], z0);
-            z1 = __ffma2_rn(p1, dn[i + k], z1);
-            h[2 * k] = h2_bits(__floats2half2_rn(p0.x, p0.y));
-            h[2 * k + 1] = h2_bits(__floats2half2_rn(p1.x, p1.y));
+            p0[k] = make_float2(ex2(x0.x), ex2(x0.y));
+            p1[k] = make_float2(ex2(x1.x), ex2(x1.y));
+            const float2 dn = *reinterpret_cast<const float2*>(&sm.tok_dn[b][8 * (i + k) + cl]);
+            z0 = __ffma2_rn(p0[k], dn, z0);
+            z1 = __ffma2_rn(p1[k], dn, z1);
           }
           // matrices: (tokens 8 i.., heads r0), (.., heads r1), (tokens 8 (i + 1).., heads r0), (.., r1)
-          stmatrix_x4(pdst + i * 1024, h[0], h[1], h[2], h[3]);
+          if constexpr (kFp4) {
+            stmatrix_x4(pdst + i * 1024, pack2(p0[0]), pack2(p1[0]), pack2(p0[1]), pack2(p1[1]));
+          } else {
+            const float4 x0 = sm.tok_r[b][8 * i + cl], y0 = sm.tok_r[b][8 * i + cl + 1];
+            const float4 x1 = sm.tok_r[b][8 * i + 8 + cl], y1 = sm.tok_r[b][8 * i + 8 + cl + 1];
+            const auto put = [&](uint32_t dst, float2 ra, float2 rb) {
+              stmatrix_x4(dst + i * 1024, pack2(__fmul2_rn(p0[0], ra)), pack2(__fmul2_rn(p1[0], ra)),
+                          pack2(__fmul2_rn(p0[1], rb)), pack2(__fmul2_rn(p1[1], rb)));
+            };
+            put(pdst, make_float2(x0.x, y0.x), make_float2(x1.x, y1.x));
+            put(pxdst, make_float2(x0.y, y0.y), make_float2(x1.y, y1.y));
+            put(pxdst + kPBytes, make_float2(x0.z, y0.z), make_float2(x1.z, y1.z));
+            put(pxdst + 2 * kPBytes, make_float2(x0.w, y0.w), make_float2(x1.w, y1.w));
+          }
         }
         l0 = z0.x + z0.y;
         l1 = z1.x + z1.y;

@@ -333,3 +333,38 @@ def test_many_rows_repeat_bit_for_bit(hcu, dev, fmt):
     some = list(range(0, rows, 97))
     lists = idx[some].cpu().numpy()
     _check(fmt, q[some].cpu(), host, list(lists), out[some], lse[some])
+
+
+@pytest.mark.parametrize("form", ["tokens", "blocks"])
+@pytest.mark.parametrize("n", [1, 33, 96, 97, 200, 500])
+def test_lse_of_short_fp8_rows(hcu, dev, form, n):
+    """lse of few tokens, whose scores' errors do not average out.  Per head: the rope is the one operand that is
+    rounded, to 11 bits (2^-12 of |q k| each); 2^-17 of all |q k| and 2e-6 for the fp32 sums and exponentials.
+    From 33 tokens on 2e-5 of itself (2-norm) as well."""
+    pool = _pool("fp8", 1024, 21)
+    rng = np.random.default_rng(n)
+    q = _q(24, 64, 22)
+    P, Q = torch.from_numpy(pool).to(dev), q.to(dev)
+    if form == "tokens":
+        lists = [rng.permutation(1024)[:n] for _ in range(24)]
+        _, lse = hcu.sparse_mla_attention(Q, P, torch.from_numpy(np.stack(lists).astype(np.int32)).to(dev), SCALE)
+    else:
+        nb = -(-n // 64)
+        table = np.stack([rng.permutation(16)[:nb] for _ in range(24)]).astype(np.int32)
+        lists = [(table[r].astype(np.int64)[:, None] * 64 + np.arange(64)).reshape(-1)[:n] for r in range(24)]
+        blocks = np.tile(np.arange(nb, dtype=np.int32), (24, 1))
+        _, lse = hcu.block_sparse_mla_attention(Q, P, torch.from_numpy(blocks).to(dev), torch.from_numpy(table).to(dev),
+                                                torch.full((24,), n, dtype=torch.int32, device=dev), SCALE)
+    z, qd = lse.double().cpu().numpy(), q.double().numpy()
+    ref, tol = [], []
+    for r in range(24):
+        v = _values("fp8", pool, lists[r])
+        s = qd[r] @ v.T * SCALE
+        every = np.abs(qd[r]) @ np.abs(v).T * SCALE
+        rope = np.abs(qd[r][:, 512:]) @ np.abs(v[:, 512:]).T * SCALE
+        tol.append((2.0 ** -12 * rope + 2.0 ** -17 * every).max(1) + 2e-6)
+        m = s.max(1, keepdims=True)
+        ref.append(m[:, 0] + np.log(np.exp(s - m).sum(1)))
+    ref = np.stack(ref)
+    assert (np.abs(z - ref) <= np.stack(tol)).all()
+    assert n < 33 or np.linalg.norm(z - ref) <= 2e-5 * np.linalg.norm(ref)
