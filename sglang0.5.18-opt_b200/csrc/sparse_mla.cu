@@ -1299,7 +1299,7 @@ __global__ __launch_bounds__(kCombineThreads) void combine_kernel(const AttnArgs
 }
 
 // CTAs: one per SM at most, no more than the parts the join holds, and two tiles each at least (one row
-// of 43 tiles: 24.6 us with 22 CTAs, 25.6 with 43, whose partials are twice as many).
+// of 43 tiles: 25.6 us with 22 CTAs, 27.6 with 43, whose partials are twice as many).
 int attn_grid(int64_t total) {
   const int64_t sms = sm_count() < kMaxParts ? sm_count() : kMaxParts, pairs = (total + 1) / 2;
   return static_cast<int>(pairs < sms ? pairs : sms);
