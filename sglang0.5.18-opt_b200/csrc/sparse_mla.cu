@@ -876,9 +876,7 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
           if (mbar_test(&sm.pready[b], (o >> 1) & 1) &&
               (none || acc != 0 || o_seg == 0 || mbar_test(&sm.oempty, (o_seg - 1) & 1))) {
             moved = true;
-            if (none) {
-              mbar_arrive(&sm.empty[b]);
-            } else {
+            if (!none) {
               tc_fence_after();
               const uint32_t id_o = idesc_f16(128, (min(kHg, p.heads - o_hg * kHg) + 15) & ~15, true);
               const uint64_t v = sw128_mnmajor_desc(smem_u32(sm.k[b]));
@@ -891,8 +889,10 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
                           (kFp4 || d == 0 ? pd : px + (((d - 1) * kPBytes) >> 4)) + ((ks * 2048) >> 4), id_o,
                           ks > 0 ? 1u : acc);
               acc = 1;
-              tc_commit(&sm.empty[b]);
             }
+            // For a tile without tokens too: the output may wait for its barrier alone, which must then stand for
+            // the products of the tiles before it.
+            tc_commit(&sm.empty[b]);
             ++o;
             if (++o_tile == p.tiles) {
               o_tile = 0;

@@ -1,0 +1,78 @@
+"""Edges of sparse_mla_attention / block_sparse_mla_attention: lists that end in whole tiles of padding."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_sparse_mla import SCALE, _check, _pool, _q
+
+pytestmark = pytest.mark.gpu
+
+TILE = 48  # candidates per tile of the kernel
+
+
+def _short_lists(rows, tiles, empty, pool, seed):
+    """int32 [rows, TILE * tiles]: random slots, the last `empty` tiles of every row and a few entries before them -1."""
+    g = np.random.default_rng(seed)
+    idx = g.integers(0, pool, (rows, TILE * tiles)).astype(np.int32)
+    valid = TILE * (tiles - empty) - g.integers(0, TILE, rows)
+    valid[::3] = TILE * (tiles - empty)  # a full last tile
+    idx[np.arange(TILE * tiles)[None] >= valid[:, None]] = -1
+    return idx
+
+
+@pytest.mark.parametrize("empty", [1, 2, 3])
+@pytest.mark.parametrize("heads", [64, 16])
+@pytest.mark.parametrize("fmt", ["fp8", "kv4"])
+def test_whole_rows_that_end_in_empty_tiles(hcu, dev, fmt, heads, empty):
+    """Rows handled whole by one CTA: the result is bit for bit that of the list cut before the empty tiles, as
+    the tiles that hold tokens are the same.  Every SM has several rows, and every run gives the same bits."""
+    rows, tiles = 4 * torch.cuda.get_device_properties(dev).multi_processor_count, 7
+    host = _pool(fmt, 4000, 31)
+    P, q = torch.from_numpy(host).to(dev), _q(rows, heads, 32)
+    Q, idx = q.to(dev), _short_lists(rows, tiles, empty, 4000, 33 + empty)
+    full = torch.from_numpy(idx).to(dev)
+    cut = torch.from_numpy(np.ascontiguousarray(idx[:, :TILE * (tiles - empty)])).to(dev)
+    out, lse = hcu.sparse_mla_attention(Q, P, cut, SCALE)
+    some = list(range(0, rows, 83))
+    _check(fmt, q[some], host, [idx[r][idx[r] >= 0] for r in some], out[some], lse[some])
+    for _ in range(20):
+        o, z = hcu.sparse_mla_attention(Q, P, full, SCALE)
+        assert torch.equal(o, out) and torch.equal(z, lse)
+
+
+@pytest.mark.parametrize("empty", [1, 2, 13])
+@pytest.mark.parametrize("fmt", ["fp8", "kv4"])
+def test_split_rows_that_end_in_empty_tiles(hcu, dev, fmt, empty):
+    """Rows shared by several CTAs, whose shares end in empty tiles or hold nothing else."""
+    sms = torch.cuda.get_device_properties(dev).multi_processor_count
+    for rows, tiles in ((sms * 2 // 3, 40), (1, 43)):
+        host = _pool(fmt, 4000, 41)
+        P, q = torch.from_numpy(host).to(dev), _q(rows, 64, 42)
+        Q, idx = q.to(dev), _short_lists(rows, tiles, empty, 4000, 43 + empty)
+        full = torch.from_numpy(idx).to(dev)
+        out, lse = hcu.sparse_mla_attention(Q, P, full, SCALE)
+        for _ in range(20):
+            o, z = hcu.sparse_mla_attention(Q, P, full, SCALE)
+            assert torch.equal(o, out) and torch.equal(z, lse)
+        some = list(range(0, rows, 7))
+        _check(fmt, q[some], host, [idx[r][idx[r] >= 0] for r in some], out[some], lse[some])
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "kv4"])
+def test_short_block_rows_end_in_empty_tiles(hcu, dev, fmt):
+    """Block form, rows shorter than the selection: visible tokens end one to three tiles before the list's end."""
+    rows, nb = 2 * torch.cuda.get_device_properties(dev).multi_processor_count, 6
+    host = _pool(fmt, 64 * 50, 51)
+    P, q = torch.from_numpy(host).to(dev), _q(rows, 64, 52)
+    g = np.random.default_rng(53)
+    table = np.stack([g.permutation(50)[:nb] for _ in range(rows)]).astype(np.int32)
+    lens = (64 * nb - TILE * g.integers(1, 4, rows) - g.integers(0, TILE, rows) * (np.arange(rows) % 2)).astype(np.int32)
+    blocks = np.tile(np.arange(nb, dtype=np.int32), (rows, 1))
+    args = [torch.from_numpy(x).to(dev) for x in (blocks, table, lens)]
+    out, lse = hcu.block_sparse_mla_attention(q.to(dev), P, *args, SCALE)
+    for _ in range(20):
+        o, z = hcu.block_sparse_mla_attention(q.to(dev), P, *args, SCALE)
+        assert torch.equal(o, out) and torch.equal(z, lse)
+    some = list(range(0, rows, 17))
+    lists = [(table[r].astype(np.int64)[:, None] * 64 + np.arange(64)).reshape(-1)[:lens[r]] for r in some]
+    _check(fmt, q[some], host, lists, out[some], lse[some])
