@@ -597,7 +597,9 @@ __device__ __forceinline__ void convert(const Raw<kFp4>& r, int sub, Conv& c) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const float x = __uint_as_float(w[g]) * dn;
-      scale[g] = __float2half2_rn(__uint_as_float((__float_as_uint(x) + 0x10000u) & 0xfffe0000u));
+      // the rounding's carry would make a zero of a NaN: what is not finite stays
+      const uint32_t xb = __float_as_uint(x), xr = (xb + 0x10000u) & 0xfffe0000u;
+      scale[g] = __float2half2_rn(__uint_as_float((~xb & 0x7f800000u) == 0 ? xb : xr));
       f = g == sub ? x : f;
       h = g == sub ? __low2float(scale[g]) : h;
     }

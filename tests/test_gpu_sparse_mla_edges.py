@@ -1,4 +1,5 @@
-"""Edges of sparse_mla_attention / block_sparse_mla_attention: lists that end in whole tiles of padding."""
+"""Edges of sparse_mla_attention / block_sparse_mla_attention: lists that end in whole tiles of padding,
+non-finite values in selected slots."""
 import numpy as np
 import pytest
 import torch
@@ -76,3 +77,42 @@ def test_short_block_rows_end_in_empty_tiles(hcu, dev, fmt):
     some = list(range(0, rows, 17))
     lists = [(table[r].astype(np.int64)[:, None] * 64 + np.arange(64)).reshape(-1)[:lens[r]] for r in some]
     _check(fmt, q[some], host, lists, out[some], lse[some])
+
+
+def _poison(fmt, slot, kind):
+    """Puts a non-finite value into one slot (uint8 [slot bytes]) in place."""
+    nan, inf = np.float32(np.nan), np.float32(np.inf)
+    put = lambda at, v: slot.__setitem__(slice(at, at + v.nbytes), np.frombuffer(v.tobytes(), np.uint8))
+    if kind == "rope":
+        put((304 if fmt == "kv4" else 528) + 14, np.uint16(0x7FC0))
+    elif fmt == "fp8":
+        if kind == "code":
+            slot[300] = 0x7F
+        else:
+            put(512 + 4 * int(kind[-1]), nan if kind.startswith("nan") else inf)
+    elif kind == "code":
+        slot[256 + 9] = 0x7F  # a group's scale
+    else:
+        put(288, nan if kind.startswith("nan") else inf)
+
+
+@pytest.mark.parametrize("fmt,kind", [("fp8", k) for k in ("nan0", "nan1", "nan2", "nan3", "inf0", "inf3", "code", "rope")] +
+                         [("kv4", k) for k in ("nan", "inf", "code", "rope")])
+def test_non_finite_slots_are_seen(hcu, dev, fmt, kind):
+    """A NaN or infinity in a selected slot makes the row's out and lse NaN, as the definition does; rows that do
+    not select the slot keep their bits."""
+    host = _pool(fmt, 1000, 61)
+    q = _q(12, 64, 62)
+    g = np.random.default_rng(63)
+    idx = g.integers(1, 1000, (12, 200)).astype(np.int32)
+    idx[4, 150:] = -1
+    clean = torch.from_numpy(host.copy()).to(dev)
+    _poison(fmt, host[0], kind)
+    P, Q = torch.from_numpy(host).to(dev), q.to(dev)
+    want, lse0 = hcu.sparse_mla_attention(Q, clean, torch.from_numpy(idx).to(dev), SCALE)
+    idx[2, 0] = idx[4, 149] = idx[7, 77] = idx[11, 199] = 0
+    out, lse = hcu.sparse_mla_attention(Q, P, torch.from_numpy(idx).to(dev), SCALE)
+    bad = [2, 4, 7, 11]
+    rest = [r for r in range(12) if r not in bad]
+    assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
+    assert torch.equal(out[rest], want[rest]) and torch.equal(lse[rest], lse0[rest])
