@@ -1275,8 +1275,8 @@ __global__ __launch_bounds__(kCombineThreads) void combine_kernel(const AttnArgs
   __syncthreads();
   m = fmaxf(fmaxf(red[sub][0], red[sub][1]), fmaxf(red[sub][2], red[sub][3]));
 #pragma unroll
-  for (int k = 0; k < kMaxParts / 128; ++k)
-    weight[sub][128 * k + t] = m == -INFINITY ? 0.f : exp2f(lse[k] - m);
+  for (int k = 0; k < kMaxParts / 128; ++k)  // an empty part weighs nothing; a NaN one shows beside empty ones too
+    weight[sub][128 * k + t] = lse[k] == -INFINITY ? 0.f : exp2f(lse[k] - m);
   __syncthreads();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;

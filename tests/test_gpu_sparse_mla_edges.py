@@ -116,3 +116,16 @@ def test_non_finite_slots_are_seen(hcu, dev, fmt, kind):
     rest = [r for r in range(12) if r not in bad]
     assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
     assert torch.equal(out[rest], want[rest]) and torch.equal(lse[rest], lse0[rest])
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "kv4"])
+def test_non_finite_slot_in_a_row_of_one_part(hcu, dev, fmt):
+    """A row split over many CTAs all of whose tokens lie in one share: the join keeps that share's NaN though every
+    other share is empty."""
+    host = _pool(fmt, 100, 64)
+    _poison(fmt, host[0], "code")
+    idx = np.full((1, 2048), -1, np.int32)
+    idx[0, 5] = 0
+    q = _q(1, 64, 65).to(dev)
+    out, lse = hcu.sparse_mla_attention(q, torch.from_numpy(host).to(dev), torch.from_numpy(idx).to(dev), SCALE)
+    assert torch.isnan(out).all() and torch.isnan(lse).all()
