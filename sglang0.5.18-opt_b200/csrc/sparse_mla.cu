@@ -586,7 +586,15 @@ __device__ __forceinline__ void convert(const Raw<kFp4>& r, int sub, Conv& c) {
   uint32_t smax = r.sc.x & 0x7fffffffu;
   if constexpr (!kFp4)
     smax = max(max(smax, r.sc.y & 0x7fffffffu), max(r.sc.z & 0x7fffffffu, r.sc.w & 0x7fffffffu));
-  c.eb = min(max(max(static_cast<int>(smax >> 23), re - 13 - kRopeShift), 27), 247);
+  // A token of zeros may take any E: 2^-64, so that its 2^-E counts into the sum of a list of any length (2^-100 with
+  // P's 2^kBias overflows it at 2^20 tokens) and its weight is no flushed one beside tokens of large latents.
+  bool zero = re == 0;
+  if constexpr (kFp4)
+    zero = zero && (smax == 0 || ((r.gs[0].x | r.gs[0].y | r.gs[0].z | r.gs[0].w | r.gs[1].x | r.gs[1].y | r.gs[1].z |
+                                   r.gs[1].w) & 0x7f7f7f7fu) == 0);
+  else
+    zero = zero && smax == 0;
+  c.eb = min(max(max(static_cast<int>(smax >> 23), re - 13 - kRopeShift), zero ? 63 : 27), 247);
   const float dn = exp2_of(254 - c.eb);
   float fr = dn * (1.f / (1 << kRopeShift));
   __half2 scale[4];

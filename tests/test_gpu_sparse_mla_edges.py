@@ -1,10 +1,10 @@
 """Edges of sparse_mla_attention / block_sparse_mla_attention: lists that end in whole tiles of padding,
-non-finite values in selected slots."""
+non-finite values and zero bytes in selected slots."""
 import numpy as np
 import pytest
 import torch
 
-from test_gpu_sparse_mla import SCALE, _check, _pool, _q
+from test_gpu_sparse_mla import SCALE, SLOT, _check, _pool, _q
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +129,33 @@ def test_non_finite_slot_in_a_row_of_one_part(hcu, dev, fmt):
     q = _q(1, 64, 65).to(dev)
     out, lse = hcu.sparse_mla_attention(q, torch.from_numpy(host).to(dev), torch.from_numpy(idx).to(dev), SCALE)
     assert torch.isnan(out).all() and torch.isnan(lse).all()
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "kv4"])
+def test_long_lists_of_zero_slots(hcu, dev, fmt):
+    """More than 2^20 slots of zero bytes per row (a cache that has not been written): every score is 0, so lse is
+    log n and out 0."""
+    rows, n = torch.cuda.get_device_properties(dev).multi_processor_count, 16400
+    kv = torch.zeros(64, 1, SLOT[fmt], dtype=torch.uint8, device=dev)
+    table = torch.zeros(1, n, dtype=torch.int32, device=dev).expand(rows, n)
+    blocks = torch.arange(n, dtype=torch.int32, device=dev).expand(rows, n)
+    lens = torch.full((rows,), 64 * n, dtype=torch.int32, device=dev)
+    out, lse = hcu.block_sparse_mla_attention(_q(rows, 8, 3).to(dev), kv, blocks, table, lens, SCALE)
+    assert (out == 0).all()
+    assert np.allclose(lse.cpu().numpy(), np.log(64.0 * n), rtol=2e-6)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "kv4"])
+def test_zero_slots_beside_large_latents(hcu, dev, fmt):
+    """Slots of zero bytes in a list with latents of order 2^48, whose scores the scale brings to order 1: the zero
+    slots' score of 0 has its full weight."""
+    host = _pool(fmt, 200, 66)
+    host[::2] = 0
+    f32 = lambda at, n: np.ascontiguousarray(host[1::2, at:at + 4 * n]).view(np.float32)
+    at, n = (512, 4) if fmt == "fp8" else (288, 1)
+    host[1::2, at:at + 4 * n] = (f32(at, n) * np.float32(2.0 ** 48)).view(np.uint8)
+    idx = np.arange(200, dtype=np.int32)[None]
+    q = _q(1, 64, 67)
+    out, lse = hcu.sparse_mla_attention(q.to(dev), torch.from_numpy(host).to(dev), torch.from_numpy(idx).to(dev),
+                                        SCALE * 2.0 ** -48)
+    _check(fmt, q, host, [idx[0]], out, lse, scale=SCALE * 2.0 ** -48)
