@@ -1400,7 +1400,7 @@ extern "C" int hcu_sparse_mla_attention(const uint16_t* q, int64_t rows, int64_t
     return HCU_ERR_ARG;
   if (rows == 0) return HCU_OK;
   if (heads > 1024 || rows > kMaxInt / 1024 || n_bt > kMaxInt / kPage || n_slots > kMaxInt) return HCU_ERR_UNSUPPORTED;
-  if (!q || !out || !lse || !workspace || (n_idx > 0 && (!indices || !kv_cache))) return HCU_ERR_ARG;
+  if (!q || !out || !lse || !workspace || (n_idx > 0 && (!indices || (n_slots > 0 && !kv_cache)))) return HCU_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv_cache) | reinterpret_cast<uintptr_t>(out) |
        reinterpret_cast<uintptr_t>(workspace)) %
       16)

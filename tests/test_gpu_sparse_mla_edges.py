@@ -159,3 +159,12 @@ def test_zero_slots_beside_large_latents(hcu, dev, fmt):
     out, lse = hcu.sparse_mla_attention(q.to(dev), torch.from_numpy(host).to(dev), torch.from_numpy(idx).to(dev),
                                         SCALE * 2.0 ** -48)
     _check(fmt, q, host, [idx[0]], out, lse, scale=SCALE * 2.0 ** -48)
+
+
+def test_empty_cache(hcu, dev):
+    """A cache without slots: a list of -1 gives the empty row, any other entry is skipped and flagged."""
+    for w in (656, 432):
+        kv = torch.empty(0, 1, w, dtype=torch.uint8, device=dev)
+        q = _q(2, 8, 1).to(dev)
+        out, lse = hcu.sparse_mla_attention(q, kv, torch.full((2, 50), -1, dtype=torch.int32, device=dev), SCALE)
+        assert (out == 0).all() and torch.isneginf(lse).all() and hcu.read_device_status() == 0
