@@ -293,8 +293,9 @@ extern "C" int hcu_select_blocks(const float* score, int64_t rows, int64_t width
   int s = 1;
   while (s < kMaxSbSplits && rows * 2 * s <= kSbFill * sm_count() && row_blocks >= 2 * s * 64) s *= 2;
   a.splits = s;
+  static_assert(32 * 1024 + sizeof(SbSmem) <= 48 * 1024, "shared memory without opt-in");
   const size_t smem = static_cast<size_t>(row_blocks) * sizeof(uint32_t);
-  if (smem > 40 * 1024) {
+  if (smem > 32 * 1024) {  // with the kernel's static part (sizeof(SbSmem)) below the 48 KB of a launch that asks for none
     const cudaError_t e = cudaFuncSetAttribute(select_blocks_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                kMaxRowBlocks * static_cast<int>(sizeof(uint32_t)));
     if (e != cudaSuccess) {
