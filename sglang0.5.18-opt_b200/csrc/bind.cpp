@@ -580,12 +580,14 @@ std::vector<torch::Tensor> step_tables(torch::Tensor& req_pages, const torch::Te
               "free_pages and free_head must be contiguous int32 [n] and [1] on req_pages' device");
   TORCH_CHECK(n_rows >= 0 && width > 0 && width % 64 == 0, "width must be a positive multiple of 64, n_rows >= 0");
   const c10::cuda::CUDAGuard guard(req_pages.device());
-  // The seven outputs share one allocation (each at a 16-byte boundary): seven of their own cost more on
-  // the host than the kernel takes.
+  // Two allocations, each output at a 16-byte boundary of its own: the two tables, and the small outputs, which
+  // must not keep the tables alive (free_head goes from step to step).  Seven allocations cost more on the host
+  // than the kernel takes.
   const int64_t rows16 = (n_rows + 3) / 4 * 4;  // int32 words of a per-row output, rounded up
-  auto base = torch::empty({n_rows * width + (n_rows * (width / 64) + 3) / 4 * 4 + 5 * rows16 + 4}, req_pages.options());
+  const auto tables = torch::empty({n_rows * width + (n_rows * (width / 64) + 3) / 4 * 4}, req_pages.options());
+  const auto small = torch::empty({5 * rows16 + 4}, req_pages.options());
   int64_t at = 0;
-  const auto carve = [&](at::IntArrayRef sizes, at::ScalarType type, int64_t words) {
+  const auto carve = [&](const torch::Tensor& base, at::IntArrayRef sizes, at::ScalarType type, int64_t words) {
     auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(),
                                                       c10::scalarTypeToTypeMeta(type));
     t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
@@ -593,13 +595,14 @@ std::vector<torch::Tensor> step_tables(torch::Tensor& req_pages, const torch::Te
     at += (words + 3) / 4 * 4;
     return t;
   };
-  const auto pt = carve({n_rows, width}, at::kInt, n_rows * width);
-  const auto bt = carve({n_rows, width / 64}, at::kInt, n_rows * (width / 64));
-  const auto loc = carve({n_rows}, at::kLong, 2 * n_rows);
-  const auto len = carve({n_rows}, at::kInt, n_rows);
-  const auto pos = carve({n_rows}, at::kInt, n_rows);
-  const auto tl = carve({n_rows}, at::kInt, n_rows);
-  const auto head = carve({1}, at::kInt, 1);
+  const auto pt = carve(tables, {n_rows, width}, at::kInt, n_rows * width);
+  const auto bt = carve(tables, {n_rows, width / 64}, at::kInt, n_rows * (width / 64));
+  at = 0;
+  const auto loc = carve(small, {n_rows}, at::kLong, 2 * n_rows);
+  const auto len = carve(small, {n_rows}, at::kInt, n_rows);
+  const auto pos = carve(small, {n_rows}, at::kInt, n_rows);
+  const auto tl = carve(small, {n_rows}, at::kInt, n_rows);
+  const auto head = carve(small, {1}, at::kInt, 1);
   check_status(hcu_step_tables(ptr<int32_t>(req_pages), req_pages.size(0), req_pages.size(1), req_pages.stride(0),
                                ptr<const int32_t>(req_idx), ptr<const int32_t>(seq_lens), ptr<const int32_t>(new_lens),
                                B, ptr<const int32_t>(free_pages), free_pages.size(0), ptr<const int32_t>(free_head),

@@ -287,7 +287,8 @@ def rope_qout_kv_store(positions, q_pe, q_out, kv_c, kv_weight, norm_eps, k_pe, 
 
 # --- sparse attention around the indexer ------------------------------------------------------------
 class StepTables(NamedTuple):
-    """What ``step_tables`` returns; the shapes are those the other ops of a step take."""
+    """What ``step_tables`` returns; the shapes are those the other ops of a step take.  The two tables share one
+    allocation and the small outputs another, so keeping a small one does not keep the tables."""
     block_table: torch.Tensor        # int32 [rows, width / 64], -1 after the request's pages
     page_table_size_1: torch.Tensor  # int32 [rows, width], -1 after the request's tokens
     lengths: torch.Tensor            # int32 [rows]: visible tokens (context_lens of mqa_logits, lengths of the top-k)
