@@ -5,8 +5,9 @@
 One layer's step for a batch of requests that bring one or two tokens each:
 
 1. ``step_tables``: pages for the new tokens, block table, slot table, lengths, slots;
-2. the new tokens' rows go into the caches: ``quant_store_index_k`` (indexer K), and the latent's slot
-   with ``rope_qout_kv_store`` (656 bytes, fp8) or ``store_mla_kv4`` (432 bytes, 4-bit);
+2. the new tokens' rows go into the caches: ``quant_store_index_k`` (indexer K), and the latent through
+   ``rope_qout_kv_store``, which norms it, rotates its rope and the queries' and writes the 656-byte fp8 slot;
+   for 432-byte 4-bit slots it is given no slot, and ``store_mla_kv4`` writes what it has normed and rotated;
 3. ``mqa_logits`` scores the context;
 4. token form: ``sparse_mask_topk_transform`` and ``sparse_mla_attention`` over the 2048 best tokens;
    block form: ``select_blocks`` and ``block_sparse_mla_attention`` over the 32 best 64-token blocks.
@@ -61,10 +62,13 @@ def make_state(requests, context, new_tokens, slots, seed=0, device="cuda"):
     for a in range(0, pages * 64, 8192):
         loc = every[a:a + 8192].contiguous()
         lat, pe = randn(loc.numel(), LATENT).to(bf), randn(loc.numel(), ROPE).to(bf)
-        write_slots(st, torch.zeros(loc.numel(), dtype=torch.int32, device=device), lat, pe, None, loc)
-    # the step's activations
-    st["kv_c"], st["k_pe"] = randn(rows, LATENT).to(bf), randn(rows, ROPE).to(bf)
-    st["q_cat"] = randn(rows, HEADS, LATENT + ROPE).to(bf)
+        q_pe = torch.zeros(loc.numel(), 1, ROPE, dtype=bf, device=device)
+        write_slots(st, torch.zeros(loc.numel(), dtype=torch.int32, device=device), lat, pe, q_pe, loc)
+    # the step's activations, and the buffers that the front end norms and rotates in place
+    st["kv_c_in"], st["k_pe_in"] = randn(rows, LATENT).to(bf), randn(rows, ROPE).to(bf)
+    st["q_cat_in"] = randn(rows, HEADS, LATENT + ROPE).to(bf)
+    for k in ("kv_c", "k_pe", "q_cat"):
+        st[k] = torch.empty_like(st[k + "_in"])
     qi = randn(rows, INDEX_HEADS * INDEX_DIM)
     qs = qi.abs().amax(1) / 448
     st["index_q"] = (qi / qs[:, None]).to(torch.float8_e4m3fn).view(rows, 1, INDEX_HEADS, INDEX_DIM)
@@ -74,19 +78,22 @@ def make_state(requests, context, new_tokens, slots, seed=0, device="cuda"):
 
 
 def write_slots(st, positions, kv_c, k_pe, q_pe, loc):
-    """The latents' slots; with fp8 slots the front end also norms the latent and rotates k_pe and q_pe."""
-    if st["slots"] == "fp8":
-        if q_pe is None:
-            q_pe = torch.zeros(kv_c.shape[0], 1, ROPE, dtype=torch.bfloat16, device=kv_c.device)
-        hcu_ops.rope_qout_kv_store(positions, q_pe, q_pe, kv_c, st["kv_weight"], 1e-6, k_pe.unsqueeze(1), st["cos_sin"],
-                                   False, st["kv"], loc)
-    else:
+    """Norms the latents, rotates k_pe and q_pe (all in place) and writes the latents' slots."""
+    fp8 = st["slots"] == "fp8"
+    # without slots (an empty loc) the front end writes none; its slot buffer is a stand-in then
+    buf, where = (st["kv"], loc) if fp8 else (kv_c.new_empty(1, 1, 656, dtype=torch.uint8), loc[:0])
+    hcu_ops.rope_qout_kv_store(positions, q_pe, q_pe, kv_c, st["kv_weight"], 1e-6, k_pe.unsqueeze(1), st["cos_sin"],
+                               False, buf, where)
+    if not fp8:
         hcu_ops.store_mla_kv4(kv_c, k_pe, loc, st["kv"])
 
 
 def decode_step(st, form="tokens", n_blocks=32):
-    """One step: returns the tables, the selection and (out, lse).  The state stays as it is, so a replay is
-    the same step again; the next one would take ``t.free_head`` and lengths raised by the new tokens."""
+    """One step: returns the tables, the selection and (out, lse).  The activations are copied to the buffers that the
+    front end works on, so the state stays as it is and a replay is the same step again; the next one would take
+    ``t.free_head`` and lengths raised by the new tokens."""
+    for k in ("kv_c", "k_pe", "q_cat"):
+        st[k].copy_(st[k + "_in"])
     t = hcu_ops.step_tables(st["req_pages"], st["req_idx"], st["seq_lens"], st["new_lens"], st["free_pages"],
                             st["free_head"], st["rows"], st["width"])
     hcu_ops.quant_store_index_k(st["index_k"], t.token_loc, st["index_cache"])
