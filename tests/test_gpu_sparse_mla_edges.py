@@ -1,10 +1,11 @@
 """Edges of sparse_mla_attention / block_sparse_mla_attention: lists that end in whole tiles of padding,
-non-finite values and zero bytes in selected slots."""
+non-finite values and zero bytes in selected slots; and bounds tight enough to see a factor left out of one 128-value
+group."""
 import numpy as np
 import pytest
 import torch
 
-from test_gpu_sparse_mla import SCALE, SLOT, _check, _pool, _q
+from test_gpu_sparse_mla import SCALE, SLOT, _check, _pool, _q, _values
 
 pytestmark = pytest.mark.gpu
 
@@ -168,3 +169,45 @@ def test_empty_cache(hcu, dev):
         q = _q(2, 8, 1).to(dev)
         out, lse = hcu.sparse_mla_attention(q, kv, torch.full((2, 50), -1, dtype=torch.int32, device=dev), SCALE)
         assert (out == 0).all() and torch.isneginf(lse).all() and hcu.read_device_status() == 0
+
+
+def _bf16_step(x):
+    return 2.0 ** (np.floor(np.log2(np.maximum(np.abs(x), 1e-30))) - 7)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "kv4"])
+def test_one_token_rows_give_the_token(hcu, dev, fmt):
+    """A row of one token returns its latent.  Its one weight is exact but for P's rounding to f16 (2^-11 at most,
+    with an fp8 group's remainder, up to 2^-7, in it), and the result is rounded to bf16 (half a step).  A
+    remainder left out of any one group breaks the bound at some of the 96 tokens."""
+    host = _pool(fmt, 96, 71)
+    q = _q(96, 64, 72)
+    idx = torch.arange(96, dtype=torch.int32, device=dev).view(96, 1)
+    out, _ = hcu.sparse_mla_attention(q.to(dev), torch.from_numpy(host).to(dev), idx, SCALE)
+    o = out.double().cpu().numpy()
+    v = _values(fmt, host, np.arange(96))[:, None, :512]
+    assert (np.abs(o - v) <= 0.5 * _bf16_step(v) * 1.02 + (2.0 ** -11 + 2.0 ** -16) * np.abs(v)).all()
+
+
+@pytest.mark.parametrize("n", [33, 200, 2048])
+@pytest.mark.parametrize("fmt", ["fp8", "kv4"])
+def test_out_of_each_group(hcu, dev, fmt, n):
+    """2-norm of out's error over all heads, per row and 128-value group, relative to out's own.  The rounding to bf16
+    is 2^-7 / sqrt(12) at most where all values are just above a power of two; weights are off by 2^-11 (P in f16) and
+    by their scores' errors, for which six deviations (2^-11 / sqrt(3) of each of 64 rope products, 1/16 x 8 in all)
+    are allowed.  The two are independent."""
+    host = _pool(fmt, 4096, 81)
+    g = np.random.default_rng(82 + n)
+    idx = np.stack([g.permutation(4096)[:n] for _ in range(12)]).astype(np.int32)
+    q = _q(12, 64, 83)
+    out, _ = hcu.sparse_mla_attention(q.to(dev), torch.from_numpy(host).to(dev), torch.from_numpy(idx).to(dev), SCALE)
+    o, qd = out.double().cpu().numpy(), q.double().numpy()
+    bound = ((2.0 ** -7 / 12 ** 0.5) ** 2 + (2.0 ** -11 + 6 * 2.0 ** -11 / 3 ** 0.5 * 0.5) ** 2) ** 0.5
+    for r in range(12):
+        v = _values(fmt, host, idx[r])
+        s = qd[r] @ v.T * SCALE
+        w = np.exp(s - s.max(1, keepdims=True))
+        ref = (w / w.sum(1, keepdims=True)) @ v[:, :512]
+        for k in range(4):
+            a, b = o[r][:, 128 * k:128 * k + 128], ref[:, 128 * k:128 * k + 128]
+            assert np.linalg.norm(a - b) <= bound * np.linalg.norm(b), (r, k)

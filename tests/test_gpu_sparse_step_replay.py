@@ -1,5 +1,6 @@
 """The example decode step (examples/sparse_decode.py) as an MLA step: the latent normed, ropes rotated in both slot
-formats; the step repeats itself, eager and in a graph."""
+formats; the step repeats itself, eager and in a graph; the new
+token takes part with its own weight."""
 import numpy as np
 import pytest
 import torch
@@ -49,3 +50,24 @@ def test_step_repeats_itself(hcu, dev, example, slots, form):  # noqa: F811
     for _ in range(3):
         g.replay()
         assert torch.equal(sel, sel2) and torch.equal(out, out2) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("slots", ["fp8", "kv4"])
+def test_new_token_has_its_own_weight(hcu, dev, example, slots):  # noqa: F811
+    """exp(lse) with the new token less exp(lse) without it is its own exp(score), within the bound of the two lse."""
+    st = example.make_state(1, 100, 1, slots)
+    t, sel, _, lse = example.decode_step(st, "tokens")
+    less = sel.clone()
+    assert sel[0, 100].item() == t.loc[0].item()
+    less[0, 100] = -1
+    _, without = hcu.sparse_mla_attention(st["q_cat"], st["kv"], less, example.SM_SCALE)
+    kv = st["kv"].cpu().numpy().reshape(st["kv"].shape[0], -1)
+    values = O.fp8_values if slots == "fp8" else O.kv4_values
+    q = st["q_cat"].double().cpu().numpy()[0]
+    s = example.SM_SCALE * (q @ values(kv[[t.loc[0].item()]])[0])
+    a, b = lse.double().cpu().numpy()[0], without.double().cpu().numpy()[0]
+    # each lse within 2^-12 of the ropes' |q k| and 2^-17 of every |q k|
+    k = np.abs(values(kv[sel[0, :101].cpu().numpy()]))
+    d = (2.0 ** -12 * (np.abs(q[:, 512:]) @ k[:, 512:].T) + 2.0 ** -17 * (np.abs(q) @ k.T)).max(1) * example.SM_SCALE + 2e-6
+    assert (np.abs((np.exp(a) - np.exp(b)) - np.exp(s)) <= np.expm1(d) * (np.exp(a) + np.exp(b))).all()
+    assert (np.exp(s) > 10 * np.expm1(d) * (np.exp(a) + np.exp(b))).any()  # a head where dropping it would show
