@@ -23,7 +23,7 @@
 //     in f16 over the tile's rope chunk, which S no longer needs.  O^T is rescaled only when a
 //     maximum has risen by more than 2^kLazy.
 // 48 tokens: Q (57 KB), two K tiles (55 KB each), three more P (18 KB, below) and the raw slots (34 KB)
-// fill the 227 KB.
+// fill the 227 KB; with 4-bit slots (one P, 23 KB of raw slots) 32 KB are free, a raw buffer's 23 among them.
 //
 // Number format.  f16 operands hold 11 bits where bf16 holds 8, and an fp8 or e2m1 value is exact in
 // f16; its range is met by powers of two taken out per token and per query row:
@@ -94,13 +94,22 @@ constexpr float kBias = 8.f;
 constexpr int kRopeShift = 10;
 constexpr int kPartFloats = kHg * kLatentDim + kHg;
 
+// What the scales of fp8 slots need beside the tile; 4-bit slots need nothing.
+template <bool kFp4>
+struct Groups {
+  uint8_t p[3][kPBytes];   // P of groups 1 to 3 (of group 0, as the only P of 4-bit slots: the tile's rope chunk)
+  float4 tok_r[2][kTile];  // what each group's scale is of its 7-bit rounding
+};
+template <>
+struct Groups<true> {};
+
+template <bool kFp4>
 struct __align__(1024) AtSmem {
   uint8_t q[(kChunks - kQTmem) * kQChunk];
   uint8_t k[2][kTileBytes];
-  uint8_t p[3][kPBytes];  // fp8: P of groups 1 to 3 (of group 0, as the only P of 4-bit slots: the tile's rope chunk)
-  __align__(128) uint8_t raw[kTile * kRawFp8];  // slots of the tile to be converted next, as they are in the cache
+  __align__(1024) Groups<kFp4> grp;
+  __align__(128) uint8_t raw[kTile * (kFp4 ? kRawFp4 : kRawFp8)];  // slots of the tile to be converted next, as they are in the cache
   __align__(16) uint8_t stage[kSoftWarps][1024];  // output rows on their way out
-  float4 tok_r[2][kTile];   // fp8: what each group's scale is of its 7-bit rounding
   float tok_e[2][kTile];    // E of each token (-inf: no token)
   float tok_up[2][kTile];   // 2^E (0: no token)
   float tok_dn[2][kTile];   // 2^-E (0: no token)
@@ -113,7 +122,7 @@ struct __align__(1024) AtSmem {
   uint32_t tmem;
   int abort;
 };
-static_assert(sizeof(AtSmem) + 1024 <= 232448, "shared memory");
+static_assert(sizeof(AtSmem<false>) + 1024 <= 232448 && sizeof(AtSmem<true>) + 1024 <= 232448, "shared memory");
 
 struct AttnArgs {
   const uint16_t* q;
@@ -645,9 +654,9 @@ __device__ __forceinline__ void convert(const Raw<kFp4>& r, int sub, Conv& c) {
 
 // Stores the warp's 8 tokens as rows 8 lw .. 8 lw + 7 of tile buffer b; on: the lane's token exists.
 template <bool kFp4>
-__device__ __forceinline__ void store_tile(AtSmem& sm, int b, int lw, int lane, bool on, const Conv& c) {
+__device__ __forceinline__ void store_tile(AtSmem<kFp4>& sm, int b, int lw, int lane, bool on, const Conv& c) {
   const int tok = lane >> 2, sub = lane & 3;
-  if constexpr (!kFp4) reinterpret_cast<float*>(&sm.tok_r[b][lw * 8 + tok])[sub] = c.rest;
+  if constexpr (!kFp4) reinterpret_cast<float*>(&sm.grp.tok_r[b][lw * 8 + tok])[sub] = c.rest;
   if (sub == 0) {
     const int t = lw * 8 + tok;
     sm.tok_e[b][t] = on ? static_cast<float>(c.eb - 127) : -INFINITY;
@@ -690,7 +699,7 @@ template <bool kFp4, bool kBlocks>
 __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_constant__ CUtensorMap map,
                                                                     const AttnArgs p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  AtSmem& sm = smem_aligned_1024<AtSmem>(smem_raw);
+  AtSmem<kFp4>& sm = smem_aligned_1024<AtSmem<kFp4>>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t f0 = first_tile(p, blockIdx.x, gridDim.x);
   const int n = static_cast<int>(first_tile(p, blockIdx.x + 1, gridDim.x) - f0);  // at least 1
@@ -890,7 +899,7 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
               tc_fence_after();
               const uint32_t id_o = idesc_f16(128, (min(kHg, p.heads - o_hg * kHg) + 15) & ~15, true);
               const uint64_t v = sw128_mnmajor_desc(smem_u32(sm.k[b]));
-              const uint64_t pd = sw32_kmajor_desc(smem_u32(sm.k[b]) + 8 * kChunk), px = sw32_kmajor_desc(smem_u32(sm.p[0]));
+              const uint64_t pd = sw32_kmajor_desc(smem_u32(sm.k[b]) + 8 * kChunk), px = sw32_kmajor_desc(smem_u32(&sm.grp));
 #pragma unroll
               for (int ks = 0; ks < kTile / 16; ++ks)
 #pragma unroll
@@ -1022,7 +1031,7 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
             tmem_ld_parts(tmem + kTmemS + 16 * j + quad, s);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              const float4 x = sm.tok_r[b][16 * j + 8 * k + cl], y = sm.tok_r[b][16 * j + 8 * k + cl + 1];
+              const float4 x = sm.grp.tok_r[b][16 * j + 8 * k + cl], y = sm.grp.tok_r[b][16 * j + 8 * k + cl + 1];
               const float2 r[4] = {make_float2(x.x, y.x), make_float2(x.y, y.y), make_float2(x.z, y.z), make_float2(x.w, y.w)};
               float2 a = make_float2(0.f, 0.f), d = a;
 #pragma unroll
@@ -1084,7 +1093,7 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
         // P: for every 16 tokens [64 heads][16 tokens], rows of 32 bytes with the 32-byte swizzle
         const int ph = 16 * warp + 8 * ((lane >> 3) & 1) + (lane & 7);
         const uint32_t pdst = smem_u32(sm.k[b]) + 8 * kChunk + st_piece(ph, lane >> 4);
-        const uint32_t pxdst = smem_u32(sm.p[0]) + st_piece(ph, lane >> 4);
+        const uint32_t pxdst = smem_u32(&sm.grp) + st_piece(ph, lane >> 4);  // grp.p
         // groups 1 to 3 have one buffer: the last tile's product has read it (the one before that came before
         // this tile's scores)
         if (!kFp4 && g > 0) mbar_wait(&sm.empty[(g - 1) & 1], ((g - 1) >> 1) & 1, abort, &g_hcu_status);
@@ -1106,8 +1115,8 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
           if constexpr (kFp4) {
             stmatrix_x4(pdst + i * 1024, pack2(p0[0]), pack2(p1[0]), pack2(p0[1]), pack2(p1[1]));
           } else {
-            const float4 x0 = sm.tok_r[b][8 * i + cl], y0 = sm.tok_r[b][8 * i + cl + 1];
-            const float4 x1 = sm.tok_r[b][8 * i + 8 + cl], y1 = sm.tok_r[b][8 * i + 8 + cl + 1];
+            const float4 x0 = sm.grp.tok_r[b][8 * i + cl], y0 = sm.grp.tok_r[b][8 * i + cl + 1];
+            const float4 x1 = sm.grp.tok_r[b][8 * i + 8 + cl], y1 = sm.grp.tok_r[b][8 * i + 8 + cl + 1];
             const auto put = [&](uint32_t dst, float2 ra, float2 rb) {
               stmatrix_x4(dst + i * 1024, pack2(__fmul2_rn(p0[0], ra)), pack2(__fmul2_rn(p1[0], ra)),
                           pack2(__fmul2_rn(p0[1], rb)), pack2(__fmul2_rn(p1[1], rb)));
@@ -1349,7 +1358,7 @@ int launch_attn(const AttnArgs& a, int grid, cudaStream_t st) {
   CUtensorMap map;
   const int rc = slot_map(&map, a, kFp4);
   if (rc != HCU_OK) return rc;
-  constexpr int smem = static_cast<int>(sizeof(AtSmem)) + 1024;
+  constexpr int smem = static_cast<int>(sizeof(AtSmem<kFp4>)) + 1024;
   cudaError_t e = cudaFuncSetAttribute(sparse_mla_kernel<kFp4, kBlocks>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
     set_last_error(e);
