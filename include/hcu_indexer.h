@@ -440,7 +440,8 @@ int hcu_topk_keys_if(const float* score, int64_t rows, int64_t width, int64_t sc
  *              (no row twice), its cached tokens, its new tokens of this step
  *   free_pages int32 [n_free]: page ids handed out in order from free_head[0]
  *   n_rows     query rows of the outputs: the new tokens, request by request; rows
- *              past sum(new_lens) are written as empty (length 0, entries -1)
+ *              past sum(new_lens) are written as empty (length 0, entries -1; the cache
+ *              writers skip and flag such a row's slot)
  *   width      tokens per row of page_table, a multiple of 64
  *   block_table int32 [n_rows, width / 64], page_table int32 [n_rows, width]
  *              (16-byte aligned): page ids and slots page * 64 + offset of the
@@ -498,10 +499,14 @@ int hcu_dequant_mla_kv4_paged(const uint8_t* kv_buffer, int64_t n_slots, int64_t
  *            writes, negative entries skipped); block b is page block_table[row, b]
  *            (int32 [rows, n_bt]) and its tokens at positions below lengths[row] count
  *   out bf16 [rows, heads, 512], lse fp32 [rows, heads]; a row without tokens gives
- *            out 0 and lse -inf
+ *            out 0 and lse -inf, a NaN in a selected slot NaN
  *   workspace >= hcu_sparse_mla_attention_workspace_bytes(rows, heads, n_idx tokens: n_idx
  *            or 64 * n_idx), 256-byte aligned, no initial contents needed
- * Slots or blocks out of range are skipped and flagged HCU_STATUS_BAD_INPUT. */
+ * Slots or blocks out of range are skipped and flagged HCU_STATUS_BAD_INPUT.
+ * Products take f16 operands and sum in fp32: latents enter exactly (groups whose scale
+ * lies 2^-14 or more below their token's largest lose bits), softmax weights are rounded to
+ * 11 bits (fewer below 2^-22 of the largest), fp8 slots' ropes to 11, query elements below
+ * 2^-18 of their head's largest lose bits.  Up to 1024 heads and 2097151 rows. */
 int64_t hcu_sparse_mla_attention_workspace_bytes(int64_t rows, int64_t heads, int64_t n_tokens);
 int hcu_sparse_mla_attention(const uint16_t* q, int64_t rows, int64_t heads, int64_t q_row, int64_t q_head,
                              const uint8_t* kv_cache, int64_t n_slots, int64_t slot_stride, int32_t kv_format,

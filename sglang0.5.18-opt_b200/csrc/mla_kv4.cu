@@ -11,10 +11,11 @@
 //
 // Both kernels are HBM streams, a warp per token and the store's lane l owning the 16 elements of
 // group l.  Bound: 1584 bytes a token each way.  70001 tokens (111 MB, 17 us at the copy rate of
-// 6.45 TB/s) take 28.6 us to store and 26.6 us to read with events around the call; 400000 tokens
-// (634 MB, 98 us) 125 and 120 us, 5.1 and 5.3 TB/s: slots of 13.5 sectors in random order are what
-// keeps them from the copy rate.  The store's arithmetic goes in pairs (packed fp32, bf16 maxima), two
-// tokens' loads ahead of it: 143 us for 400000 with one element an instruction and one token a warp.
+// 6.45 TB/s) take 28.7 us to store and 26.7 us to read with L2 flushed and events around the call, 22.2 and 21.4 in
+// a graph of launches; 400000 tokens (634 MB, 98 us) 125 and 119 us, 116 and 114 in a graph, 5.5 TB/s.  The random
+// order of the slots is a smaller part of what keeps them from the copy rate: in order 109 and 107 us.  The
+// store's arithmetic goes in pairs (packed fp32, bf16 maxima), two tokens' loads ahead of it: 143 us for
+// 400000 with one element an instruction and one token a warp.
 #include <cuda_fp4.h>
 #include <cuda_fp8.h>
 

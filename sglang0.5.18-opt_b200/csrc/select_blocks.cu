@@ -13,8 +13,9 @@
 // the SMs S is 1 and the select of one row overlaps the streams of the others on its SM.
 //
 // Bound: the read of the scores, 4 B + 1 bit per visible token.  4096 rows of 67K tokens (1.14 GB, 177 us
-// at the copy rate of 6.45 TB/s) take 209 us, 5.5 TB/s.  128 rows of 4K to 64K tokens (18 MB, 2.9 us)
-// take 12 us: launch, the cluster's two barriers and the select's passes, each a few barriers long.
+// at the copy rate of 6.45 TB/s) take 208 us in a graph of launches, 5.5 TB/s, and 225 as one call with L2 flushed.
+// 128 rows of 4K to 64K tokens (18 MB, 2.9 us) take 12.8 us in a graph: the cluster's two barriers and the
+// select's passes, each a few barriers long, stand around the stream; their shares have not been measured apart.
 #include <cooperative_groups.h>
 
 #include "common.cuh"

@@ -37,6 +37,7 @@
 // r = 1 +- 2^-8, is put in where a group's sums are: S has a part per 128-value group, s = sum_g r_g S_g in
 // fp32, and block g of O^T takes P r_g, a P of its own.  The rope joins S_3, divided by r_3: the one
 // operand that is rounded (2^-12 each).  lse of 33 tokens is 8e-6 of itself off, of 2048 tokens 8e-7.
+// A scale that is not finite is not rounded: its NaN or infinity goes through the products into the row.
 //
 // S * 2^(E + e) is the score; P carries 2^E of its token in its exponent (w = s + E, whose maximum is
 // the running one), so O needs no correction, and the sum takes 2^-E back per token.
@@ -48,8 +49,8 @@
 // S 940, softmax 1250 with one P, O 430 cycles), with two K tiles and one of raw slots to overlap it.  Both
 // were traded, with one P: a third K tile took 7 % longer, a second raw buffer 11 %, copies of 16 bytes from
 // the loader warps in place of the raw ring 14 to 19 %.  2048 rows x 64 heads x 2048 fp8 tokens (584 GFLOP)
-// take 1.28 ms, 456 TFLOP/s (1.015 with rounded scales, one S and one P); 128 rows 103 us; one row 26 us;
-// 192 rows of 4-bit slots 138 us.  L2 flushed before each call.
+// take 1.30 ms, 447 TFLOP/s (1.015 ms with rounded scales, one S and one P); 128 rows 104 us; one row 28 us;
+// 192 rows of 4-bit slots 136 us.  L2 flushed before each call; in a graph of launches 1.30 ms, 99, 21 and 129 us.
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 

@@ -304,9 +304,10 @@ def step_tables(req_pages, req_idx, seq_lens, new_lens, free_pages, free_head, n
     Request ``i`` of the step is row ``req_idx[i]`` of ``req_pages`` (int32 ``[requests, max_pages]``, page ids
     of 64 tokens), has ``seq_lens[i]`` cached tokens and brings ``new_lens[i]`` new ones (all int32).  The pages
     that the new tokens need come from ``free_pages`` in order, from ``free_head[0]`` on, and are written into
-    ``req_pages`` in place; the returned ``free_head`` is the next step's.  The query rows are the new tokens, request by request; ``n_rows`` may exceed their
-    number (a padded batch): the rows after them are empty (length 0, entries -1).  ``width`` (a multiple of 64)
-    is the tokens per row of the tables.  Nothing is read on the host, so a step can be captured in a CUDA graph;
+    ``req_pages`` in place; the returned ``free_head`` is the next step's.  The query rows are the new tokens, request
+    by request; ``n_rows`` may exceed their number (a padded batch): the rows after them are empty (length 0, entries
+    -1; the cache writers skip their slot of -1, but set status bit 2 for it).  ``width`` (a multiple of 64) is the
+    tokens per row of the tables.  Nothing is read on the host, so a step can be captured in a CUDA graph;
     pages that run out, requests that outgrow the tables and bad lengths give -1 entries and set the device
     status bit 2 (``read_device_status``)."""
     return StepTables(*_C.step_tables(req_pages, req_idx, seq_lens, new_lens, free_pages, free_head, int(n_rows),
@@ -329,7 +330,12 @@ def sparse_mla_attention(q, kv_cache, indices, sm_scale):
 
     ``kv_cache``: uint8 ``[slots, 1, 656]`` (``rope_qout_kv_store``) or ``[slots, 1, 432]``
     (``store_mla_kv4``).  Returns ``(out, lse)``: bf16 ``[rows, heads, 512]`` = softmax(sm_scale q k) k[:512] and
-    float32 ``[rows, heads]`` = log sum exp; a row without tokens gives 0 and -inf."""
+    float32 ``[rows, heads]`` = log sum exp; a row without tokens gives 0 and -inf, a NaN in a selected slot NaN.
+
+    Products take f16 operands (11 bits) and sum in float32.  Latents enter exactly; rounded are the softmax weights
+    (2^-11; below 2^-22 of a row's largest fewer bits), the ropes of fp8 slots, query elements below 2^-18 of their
+    head's largest, and latents of a group whose scale lies 2^-14 or more below the token's largest.  ``lse`` is off by
+    about 1e-5 of itself at 33 tokens and 1e-6 at 2048, ``out`` by 2^-11 beside its rounding to bf16."""
     return tuple(_C.sparse_mla_attention(q, kv_cache, indices, None, None, float(sm_scale)))
 
 
