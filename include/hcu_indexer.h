@@ -503,10 +503,10 @@ int hcu_dequant_mla_kv4_paged(const uint8_t* kv_buffer, int64_t n_slots, int64_t
  *   workspace >= hcu_sparse_mla_attention_workspace_bytes(rows, heads, n_idx tokens: n_idx
  *            or 64 * n_idx), 256-byte aligned, no initial contents needed
  * Slots or blocks out of range are skipped and flagged HCU_STATUS_BAD_INPUT.
- * Products take f16 operands and sum in fp32: latents enter exactly (groups whose scale
- * lies 2^-14 or more below their token's largest lose bits), softmax weights are rounded to
- * 11 bits (fewer below 2^-22 of the largest), fp8 slots' ropes to 11, query elements below
- * 2^-18 of their head's largest lose bits.  Up to 1024 heads and 2097151 rows. */
+ * Products take f16 operands and sum in fp32: latents and ropes enter exactly (fp8 slots'
+ * ropes to 2^-18; groups whose scale lies 2^-14 or more below their token's largest lose
+ * bits), softmax weights are rounded to 11 bits (fewer below 2^-22 of the largest), query
+ * elements below 2^-18 of their head's largest lose bits.  Up to 1024 heads and 2097151 rows. */
 int64_t hcu_sparse_mla_attention_workspace_bytes(int64_t rows, int64_t heads, int64_t n_tokens);
 int hcu_sparse_mla_attention(const uint16_t* q, int64_t rows, int64_t heads, int64_t q_row, int64_t q_head,
                              const uint8_t* kv_cache, int64_t n_slots, int64_t slot_stride, int32_t kv_format,

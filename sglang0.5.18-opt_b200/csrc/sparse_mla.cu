@@ -13,7 +13,8 @@
 //     ahead, and copies them into the raw buffer, four slots per TMA gather;
 //   * 6 loader warps (one 8-token swizzle group each) read the raw slots, convert them to f16 in
 //     registers, which frees the raw buffer, and store them as the tile's K once a K buffer is free: 9
-//     chunks of [48 tokens][64 values], rows of 128 bytes, 128-byte swizzle.  A chunk is a K-major
+//     chunks of [48 tokens][64 values], rows of 128 bytes, 128-byte swizzle; for fp8 slots a tenth, the
+//     rope's second operand, whose one buffer is free, and filled, earlier: as soon as the last tile's S is there.  A chunk is a K-major
 //     operand for q k^T and, read the other way, an MN-major one for v^T, so the latent is stored once;
 //   * 4 warps bring each segment's Q in as f16: two chunks to TMEM, seven to shared memory;
 //   * the MMA thread issues S = Q K^T (M = 64 heads, N = 48 tokens, K = 576) and, up to two tiles
@@ -22,8 +23,8 @@
 //   * 4 softmax warps (16 heads each) read S, keep the running maximum and sum in fp32 and write P
 //     in f16 over the tile's rope chunk, which S no longer needs.  O^T is rescaled only when a
 //     maximum has risen by more than 2^kLazy.
-// 48 tokens: Q (57 KB), two K tiles (55 KB each), three more P (18 KB, below) and the raw slots (34 KB)
-// fill the 227 KB; with 4-bit slots (one P, 23 KB of raw slots) 32 KB are free, a raw buffer's 23 among them.
+// 48 tokens: Q (57 KB), two K tiles (55 KB each), three more P (18 KB, below), a tenth chunk (6 KB) and the raw
+// slots (34 KB) fill the 227 KB; with 4-bit slots (one P, 23 KB of raw slots) 32 KB are free, a raw buffer's 23 among them.
 //
 // Number format.  f16 operands hold 11 bits where bf16 holds 8, and an fp8 or e2m1 value is exact in
 // f16; its range is met by powers of two taken out per token and per query row:
@@ -35,9 +36,11 @@
 // fp8 group's scale has 24, and rounded products put lse of 33 tokens 5e-5 of itself off.  So scales are
 // rounded to 7 bits, whose products with a value's 4 are exact, and what a scale is of its rounding,
 // r = 1 +- 2^-8, is put in where a group's sums are: S has a part per 128-value group, s = sum_g r_g S_g in
-// fp32, and block g of O^T takes P r_g, a P of its own.  The rope joins S_3, divided by r_3: the one
-// operand that is rounded (2^-12 each).  lse of 33 tokens is 8e-6 of itself off, of 2048 tokens 8e-7.
-// A scale that is not finite is not rounded: its NaN or infinity goes through the products into the row.
+// fp32, and block g of O^T takes P r_g, a P of its own.  The rope joins S_3 as two operands that make rope / r_3:
+// the rope, exact, and rope * (1 / r_3 - 1), at most 2^-7 of it and rounded (2^-18 of the rope; the quotient
+// as one operand, rounded by 2^-12, put lse of 33 tokens 8e-6 off).  lse of 33 tokens is 1.3e-7 of itself off,
+// of 2048 tokens 7e-8, as with 4-bit slots.  A scale that is not finite is not rounded: its NaN or infinity goes
+// through the products into the row.
 //
 // S * 2^(E + e) is the score; P carries 2^E of its token in its exponent (w = s + E, whose maximum is
 // the running one), so O needs no correction, and the sum takes 2^-E back per token.
@@ -49,8 +52,8 @@
 // S 940, softmax 1250 with one P, O 430 cycles), with two K tiles and one of raw slots to overlap it.  Both
 // were traded, with one P: a third K tile took 7 % longer, a second raw buffer 11 %, copies of 16 bytes from
 // the loader warps in place of the raw ring 14 to 19 %.  2048 rows x 64 heads x 2048 fp8 tokens (584 GFLOP)
-// take 1.30 ms, 447 TFLOP/s (1.015 ms with rounded scales, one S and one P); 128 rows 104 us; one row 28 us;
-// 192 rows of 4-bit slots 136 us.  L2 flushed before each call; in a graph of launches 1.30 ms, 99, 21 and 129 us.
+// take 1.27 ms, 460 TFLOP/s (1.015 ms with rounded scales, one S and one P); 128 rows 103 us; one row 28 us;
+// 192 rows of 4-bit slots 136 us.  L2 flushed before each call; in a graph of launches 1.26 ms, 96, 21 and 129 us.
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 
@@ -95,14 +98,18 @@ constexpr float kBias = 8.f;
 constexpr int kRopeShift = 10;
 constexpr int kPartFloats = kHg * kLatentDim + kHg;
 
-// What the scales of fp8 slots need beside the tile; 4-bit slots need nothing.
+// What the scales of fp8 slots need beside the tile.  Output rows on their way out (kSoftWarps KB) have the first
+// bytes, of P where there is one: a segment's last product has read it by then, its writers are the same warps.
 template <bool kFp4>
 struct Groups {
   uint8_t p[3][kPBytes];   // P of groups 1 to 3 (of group 0, as the only P of 4-bit slots: the tile's rope chunk)
+  uint8_t rest[kChunk];    // the rope's second operand
   float4 tok_r[2][kTile];  // what each group's scale is of its 7-bit rounding
 };
 template <>
-struct Groups<true> {};
+struct Groups<true> {
+  uint8_t stage[kSoftWarps * 1024];
+};
 
 template <bool kFp4>
 struct __align__(1024) AtSmem {
@@ -110,7 +117,6 @@ struct __align__(1024) AtSmem {
   uint8_t k[2][kTileBytes];
   __align__(1024) Groups<kFp4> grp;
   __align__(128) uint8_t raw[kTile * (kFp4 ? kRawFp4 : kRawFp8)];  // slots of the tile to be converted next, as they are in the cache
-  __align__(16) uint8_t stage[kSoftWarps][1024];  // output rows on their way out
   float tok_e[2][kTile];    // E of each token (-inf: no token)
   float tok_up[2][kTile];   // 2^E (0: no token)
   float tok_dn[2][kTile];   // 2^-E (0: no token)
@@ -584,6 +590,7 @@ __device__ __forceinline__ float convert_q(const AttnArgs& p, uint32_t q, float*
 struct Conv {
   uint32_t y[8][8];  // latent elements 64 i + 16 sub .. + 15, two f16 a word
   uint32_t r[8];     // rope
+  uint32_t dr;       // fp8: 1 / r_3 - 1 twice, 0 for a token with an infinite rope, whose products that leaves as they are
   int eb;            // biased exponent taken out of the token
   float rest;        // fp8: group sub's scale over its rounding
 };
@@ -606,7 +613,7 @@ __device__ __forceinline__ void convert(const Raw<kFp4>& r, int sub, Conv& c) {
     zero = zero && smax == 0;
   c.eb = min(max(max(static_cast<int>(smax >> 23), re - 13 - kRopeShift), zero ? 63 : 27), 247);
   const float dn = exp2_of(254 - c.eb);
-  float fr = dn * (1.f / (1 << kRopeShift));
+  const float fr = dn * (1.f / (1 << kRopeShift));
   __half2 scale[4];
   if constexpr (!kFp4) {
     // scales to 7 bits, so that their products with an fp8 value's 4 are exact in f16's 11
@@ -622,8 +629,8 @@ __device__ __forceinline__ void convert(const Raw<kFp4>& r, int sub, Conv& c) {
       h = g == sub ? __low2float(scale[g]) : h;
     }
     c.rest = h != 0.f ? __fdividef(f, h) : 1.f;  // h is 0 where the group is 2^-25 of the token's largest
-    // the rope shares group 3's part of the score
-    fr = __fdividef(fr, __shfl_sync(0xffffffffu, c.rest, (threadIdx.x & 31) | 3));
+    const float r3 = __shfl_sync(0xffffffffu, c.rest, (threadIdx.x & 31) | 3);
+    c.dr = re == 255 ? 0u : h2_bits(__float2half2_rn(__fdividef(1.f - r3, r3)));
   }
   const uint32_t rw[8] = {r.rope[0].x, r.rope[0].y, r.rope[0].z, r.rope[0].w,
                           r.rope[1].x, r.rope[1].y, r.rope[1].z, r.rope[1].w};
@@ -673,6 +680,18 @@ __device__ __forceinline__ void store_tile(AtSmem<kFp4>& sm, int b, int lw, int 
   });
   st_shared_v4<8 * kChunk>(p0, c.r[0], c.r[1], c.r[2], c.r[3]);
   st_shared_v4<8 * kChunk>(p1, c.r[4], c.r[5], c.r[6], c.r[7]);
+}
+
+// The rope's second operand for the same tokens.
+__device__ __forceinline__ void store_rest(uint32_t base, int lw, int lane, const Conv& c) {
+  const int tok = lane >> 2, sub = lane & 3;
+  const uint32_t p0 = base + lw * 1024 + tok * 128 + (((2 * sub) ^ tok) << 4), p1 = p0 ^ 16u;
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    h[i] = c.dr == 0 ? 0u : h2_bits(__hmul2(*reinterpret_cast<const __half2*>(&c.r[i]), *reinterpret_cast<const __half2*>(&c.dr)));
+  st_shared_v4(p0, h[0], h[1], h[2], h[3]);
+  st_shared_v4(p1, h[4], h[5], h[6], h[7]);
 }
 
 // Walks the tiles of a CTA's range.
@@ -763,6 +782,14 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
       } else {
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.rempty);
+      }
+      if constexpr (!kFp4) {
+        if (some) {
+          // One buffer: the scores of the tiles before have been formed (also when the last tile held no token).
+          // Stored here it costs nothing; after the tile, where S waits for it, 7 % (2048 rows: 1273 and 1365 us).
+          if (g > 0) mbar_wait(&sm.sfull[(g - 1) & 1], ((g - 1) >> 1) & 1, abort, &g_hcu_status);
+          store_rest(smem_u32(sm.grp.rest), lw, lane, conv);
+        }
       }
       if (g >= 2) mbar_wait(&sm.empty[b], ((g >> 1) - 1) & 1, abort, &g_hcu_status);
       if (some) {
@@ -874,10 +901,17 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
                 else
                   mma_f16(d, qd + (((c - kQTmem) * kQChunk + off) >> 4), kd + ((c * kChunk + off) >> 4), id_s, add);
               }
+              if constexpr (!kFp4) {
+                const uint64_t ld = sw128_kmajor_desc(smem_u32(sm.grp.rest));
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k)
+                  mma_f16(tmem + kTmemS + kTile * 3, qd + (((kChunks - 1 - kQTmem) * kQChunk + 32 * k) >> 4), ld + (32 * k >> 4),
+                          id_s, 1u);
+              }
               tc_commit(&sm.sfull[b]);
             } else {
               s_none |= 1u << b;
-              mbar_arrive(&sm.sfull[b]);
+              tc_commit(&sm.sfull[b]);  // stands for the scores of the tiles before, like any other tile's
             }
             ++s;
             if (++s_tile == p.tiles) {
@@ -1169,7 +1203,7 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
         if (whole) {
           // 16 latent values x 32 heads at a time: fragments, transposed into the warp's 1 KB as rows of
           // 32 bytes per head, then stored as whole sectors
-          const uint32_t st = smem_u32(sm.stage[warp]);
+          const uint32_t st = smem_u32(&sm.grp) + 1024 * warp;
           uint16_t* dst = p.out + (row * p.heads + h0) * kLatentDim + 32 * warp + 8 * (lane & 1);
           const int piece = st_piece(lane >> 1, lane & 1);
 #pragma unroll 1

@@ -332,10 +332,10 @@ def sparse_mla_attention(q, kv_cache, indices, sm_scale):
     (``store_mla_kv4``).  Returns ``(out, lse)``: bf16 ``[rows, heads, 512]`` = softmax(sm_scale q k) k[:512] and
     float32 ``[rows, heads]`` = log sum exp; a row without tokens gives 0 and -inf, a NaN in a selected slot NaN.
 
-    Products take f16 operands (11 bits) and sum in float32.  Latents enter exactly; rounded are the softmax weights
-    (2^-11; below 2^-22 of a row's largest fewer bits), the ropes of fp8 slots, query elements below 2^-18 of their
-    head's largest, and latents of a group whose scale lies 2^-14 or more below the token's largest.  ``lse`` is off by
-    about 1e-5 of itself at 33 tokens and 1e-6 at 2048, ``out`` by 2^-11 beside its rounding to bf16."""
+    Products take f16 operands (11 bits) and sum in float32.  Latents and ropes enter exactly (the ropes of fp8 slots to
+    2^-18); rounded are the softmax weights (2^-11; below 2^-22 of a row's largest fewer bits), query elements below
+    2^-18 of their head's largest, and latents of a group whose scale lies 2^-14 or more below the token's largest.
+    ``lse`` is off by about 1e-7 of itself, ``out`` by 2^-11 beside its rounding to bf16."""
     return tuple(_C.sparse_mla_attention(q, kv_cache, indices, None, None, float(sm_scale)))
 
 

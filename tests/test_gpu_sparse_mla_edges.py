@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import sparse as O
 from test_gpu_sparse_mla import SCALE, SLOT, _check, _pool, _q, _values
 
 pytestmark = pytest.mark.gpu
@@ -120,6 +121,24 @@ def test_non_finite_slots_are_seen(hcu, dev, fmt, kind):
 
 
 @pytest.mark.parametrize("fmt", ["fp8", "kv4"])
+def test_infinite_rope(hcu, dev, fmt):
+    """An infinite rope element scores +inf in heads whose query element is positive, which gives NaN, and -inf where it
+    is negative: there the slot has no weight, and the result is that of the list without it."""
+    host = _pool(fmt, 300, 68)
+    at = (304 if fmt == "kv4" else 528) + 14
+    host[0, at:at + 2] = np.frombuffer(np.uint16(0x7F80).tobytes(), np.uint8)
+    q = _q(3, 64, 69)
+    idx = np.random.default_rng(70).integers(1, 300, (3, 130)).astype(np.int32)
+    idx[:, 60] = 0
+    out, lse = hcu.sparse_mla_attention(q.to(dev), torch.from_numpy(host).to(dev), torch.from_numpy(idx).to(dev), SCALE)
+    for r in range(3):
+        up = q[r, :, 512 + 7] > 0
+        assert torch.isnan(out[r, up.to(dev)]).all() and torch.isnan(lse[r, up.to(dev)]).all()
+        rest = (~up).to(dev)
+        _check(fmt, q[r:r + 1, ~up], host, [idx[r][idx[r] > 0]], out[r:r + 1, rest], lse[r:r + 1, rest])
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "kv4"])
 def test_non_finite_slot_in_a_row_of_one_part(hcu, dev, fmt):
     """A row split over many CTAs all of whose tokens lie in one share: the join keeps that share's NaN though every
     other share is empty."""
@@ -211,3 +230,45 @@ def test_out_of_each_group(hcu, dev, fmt, n):
         for k in range(4):
             a, b = o[r][:, 128 * k:128 * k + 128], ref[:, 128 * k:128 * k + 128]
             assert np.linalg.norm(a - b) <= bound * np.linalg.norm(b), (r, k)
+
+
+@pytest.mark.parametrize("form", ["tokens", "blocks"])
+@pytest.mark.parametrize("n", [33, 50, 100, 200, 500, 2048])
+@pytest.mark.parametrize("fmt", ["fp8", "kv4"])
+def test_lse_is_that_of_32_bit_products(hcu, dev, fmt, n, form):
+    """No operand of the scores is rounded by more than 2^-18 (a rope of an fp8 slot goes in as two f16 terms), so lse is off by what 40 steps of 32-bit accumulation leave, 2^-23 of the running sum each: for scores up to 8 about
+    sqrt(40) 2^-23 8 = 6e-6 a score, over at least five tokens of weight 2.7e-6, of an lse of 4 or more 7e-7.  1e-6 of
+    itself is allowed (2-norm)."""
+    rows, heads = 24, 64
+    g = torch.Generator().manual_seed(91)
+    lat, rope = torch.randn(2048, 512, generator=g).bfloat16(), torch.randn(2048, 64, generator=g).bfloat16()
+    u = lambda t: t.contiguous().view(torch.int16).numpy().view(np.uint16)
+    if fmt == "kv4":
+        host = O.kv4_pack(u(lat), u(rope))
+    else:
+        x = lat.float().view(2048, 4, 128)
+        sc = (x.abs().amax(-1) / 448).float()
+        codes = (x / sc[..., None]).to(torch.float8_e4m3fn).view(2048, 512).view(torch.uint8).numpy()
+        host = np.concatenate([codes, sc.contiguous().view(torch.uint8).numpy().reshape(2048, 16),
+                               u(rope).view(np.uint8).reshape(2048, 128)], 1)
+    rng = np.random.default_rng(92 + n)
+    q = _q(rows, heads, 93)
+    P, Q = torch.from_numpy(host).to(dev), q.to(dev)
+    if form == "tokens":
+        lists = [rng.permutation(2048)[:n] for _ in range(rows)]
+        _, lse = hcu.sparse_mla_attention(Q, P, torch.from_numpy(np.stack(lists).astype(np.int32)).to(dev), SCALE)
+    else:
+        nb = -(-n // 64)
+        table = np.stack([rng.permutation(32)[:nb] for _ in range(rows)]).astype(np.int32)
+        lists = [(table[r].astype(np.int64)[:, None] * 64 + np.arange(64)).reshape(-1)[:n] for r in range(rows)]
+        blocks = np.tile(np.arange(nb, dtype=np.int32), (rows, 1))
+        _, lse = hcu.block_sparse_mla_attention(Q, P, torch.from_numpy(blocks).to(dev), torch.from_numpy(table).to(dev),
+                                                torch.full((rows,), n, dtype=torch.int32, device=dev), SCALE)
+    z, qd = lse.double().cpu().numpy(), q.double().numpy()
+    ref = []
+    for r in range(rows):
+        s = qd[r] @ _values(fmt, host, lists[r]).T * SCALE
+        m = s.max(1, keepdims=True)
+        ref.append(m[:, 0] + np.log(np.exp(s - m).sum(1)))
+    ref = np.stack(ref)
+    assert np.linalg.norm(z - ref) <= 1e-6 * np.linalg.norm(ref)
