@@ -45,11 +45,11 @@
 // S * 2^(E + e) is the score; P carries 2^E of its token in its exponent (w = s + E, whose maximum is
 // the running one), so O needs no correction, and the sum takes 2^-E back per token.
 //
-// Bound.  A 48-token tile needs 1370 cycles of the tensor pipe (940 for S, whose M of 64 fills half of
-// it, 430 for O) and about 2500 of the shared-memory port at 128 B per cycle (34 KB of raw slots in and
-// out, 55 KB of K and 24 KB of P in, 110 KB of Q and K operands for S, 72 KB of V and P for O); it takes
-// 4100 (fp8).  What is left is the chain of a tile through its warps (copy 2900, convert 650, store 1000,
-// S 940, softmax 1250 with one P, O 430 cycles), with two K tiles and one of raw slots to overlap it.  Both
+// Bound.  A 48-token fp8 tile needs 1340 cycles of the tensor pipe (960 for S, whose M of 64 fills half of
+// it, 380 for O) and about 2700 of the shared-memory port at 128 B per cycle (34 KB of raw slots in and
+// out, 61 KB of K and 24 KB of P in, 124 KB of Q and K operands for S, 72 KB of V and P for O); it takes
+// 4100.  What is left is the chain of a tile through its warps (copy 2900, convert 650, store 1000,
+// S 960, softmax 1250 with one P, O 380 cycles), with two K tiles and one of raw slots to overlap it.  Both
 // were traded, with one P: a third K tile took 7 % longer, a second raw buffer 11 %, copies of 16 bytes from
 // the loader warps in place of the raw ring 14 to 19 %.  2048 rows x 64 heads x 2048 fp8 tokens (584 GFLOP)
 // take 1.27 ms, 460 TFLOP/s (1.015 ms with rounded scales, one S and one P); 128 rows 103 us; one row 28 us;
