@@ -14,8 +14,9 @@
 //   * 6 loader warps (one 8-token swizzle group each) read the raw slots, convert them to f16 in
 //     registers, which frees the raw buffer, and store them as the tile's K once a K buffer is free: 9
 //     chunks of [48 tokens][64 values], rows of 128 bytes, 128-byte swizzle; for fp8 slots a tenth, the
-//     rope's second operand, whose one buffer is free, and filled, earlier: as soon as the last tile's S is there.  A chunk is a K-major
-//     operand for q k^T and, read the other way, an MN-major one for v^T, so the latent is stored once;
+//     rope's second operand, whose one buffer is free, and filled, earlier: once the last tile's S is there.
+//     A chunk is a K-major operand for q k^T and, read the other way, an MN-major one for v^T, so the
+//     latent is stored once;
 //   * 4 warps bring each segment's Q in as f16: two chunks to TMEM, seven to shared memory;
 //   * the MMA thread issues S = Q K^T (M = 64 heads, N = 48 tokens, K = 576) and, up to two tiles
 //     behind, O^T += V^T P^T (M = 128 latent values x 4, N = heads, K = 48 tokens): with the latent as M
@@ -24,7 +25,7 @@
 //     in f16 over the tile's rope chunk, which S no longer needs.  O^T is rescaled only when a
 //     maximum has risen by more than 2^kLazy.
 // 48 tokens: Q (57 KB), two K tiles (55 KB each), three more P (18 KB, below), a tenth chunk (6 KB) and the raw
-// slots (34 KB) fill the 227 KB; with 4-bit slots (one P, 23 KB of raw slots) 32 KB are free, a raw buffer's 23 among them.
+// slots (34 KB) fill the 227 KB; with 4-bit slots (one P, 23 KB of raw slots) 32 KB are free.
 //
 // Number format.  f16 operands hold 11 bits where bf16 holds 8, and an fp8 or e2m1 value is exact in
 // f16; its range is met by powers of two taken out per token and per query row:
@@ -116,7 +117,8 @@ struct __align__(1024) AtSmem {
   uint8_t q[(kChunks - kQTmem) * kQChunk];
   uint8_t k[2][kTileBytes];
   __align__(1024) Groups<kFp4> grp;
-  __align__(128) uint8_t raw[kTile * (kFp4 ? kRawFp4 : kRawFp8)];  // slots of the tile to be converted next, as they are in the cache
+  // slots of the tile to be converted next, as they are in the cache
+  __align__(128) uint8_t raw[kTile * (kFp4 ? kRawFp4 : kRawFp8)];
   float tok_e[2][kTile];    // E of each token (-inf: no token)
   float tok_up[2][kTile];   // 2^E (0: no token)
   float tok_dn[2][kTile];   // 2^-E (0: no token)
@@ -590,7 +592,7 @@ __device__ __forceinline__ float convert_q(const AttnArgs& p, uint32_t q, float*
 struct Conv {
   uint32_t y[8][8];  // latent elements 64 i + 16 sub .. + 15, two f16 a word
   uint32_t r[8];     // rope
-  uint32_t dr;       // fp8: 1 / r_3 - 1 twice, 0 for a token with an infinite rope, whose products that leaves as they are
+  uint32_t dr;       // fp8: 1 / r_3 - 1, twice; 0 (no second operand) beside an infinite rope, which it could make a NaN
   int eb;            // biased exponent taken out of the token
   float rest;        // fp8: group sub's scale over its rounding
 };
@@ -689,7 +691,8 @@ __device__ __forceinline__ void store_rest(uint32_t base, int lw, int lane, cons
   uint32_t h[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    h[i] = c.dr == 0 ? 0u : h2_bits(__hmul2(*reinterpret_cast<const __half2*>(&c.r[i]), *reinterpret_cast<const __half2*>(&c.dr)));
+    h[i] = c.dr == 0 ? 0u
+                     : h2_bits(__hmul2(*reinterpret_cast<const __half2*>(&c.r[i]), *reinterpret_cast<const __half2*>(&c.dr)));
   st_shared_v4(p0, h[0], h[1], h[2], h[3]);
   st_shared_v4(p1, h[4], h[5], h[6], h[7]);
 }
@@ -905,8 +908,8 @@ __global__ __launch_bounds__(kAtThreads, 1) void sparse_mla_kernel(const __grid_
                 const uint64_t ld = sw128_kmajor_desc(smem_u32(sm.grp.rest));
 #pragma unroll
                 for (uint32_t k = 0; k < 4; ++k)
-                  mma_f16(tmem + kTmemS + kTile * 3, qd + (((kChunks - 1 - kQTmem) * kQChunk + 32 * k) >> 4), ld + (32 * k >> 4),
-                          id_s, 1u);
+                  mma_f16(tmem + kTmemS + kTile * 3, qd + (((kChunks - 1 - kQTmem) * kQChunk + 32 * k) >> 4),
+                          ld + (32 * k >> 4), id_s, 1u);
               }
               tc_commit(&sm.sfull[b]);
             } else {

@@ -236,7 +236,8 @@ def test_out_of_each_group(hcu, dev, fmt, n):
 @pytest.mark.parametrize("n", [33, 50, 100, 200, 500, 2048])
 @pytest.mark.parametrize("fmt", ["fp8", "kv4"])
 def test_lse_is_that_of_32_bit_products(hcu, dev, fmt, n, form):
-    """No operand of the scores is rounded by more than 2^-18 (a rope of an fp8 slot goes in as two f16 terms), so lse is off by what 40 steps of 32-bit accumulation leave, 2^-23 of the running sum each: for scores up to 8 about
+    """No operand of the scores is rounded by more than 2^-18 (a rope of an fp8 slot goes in as two f16 terms), so lse is
+    off by what 40 steps of 32-bit accumulation leave, 2^-23 of the running sum each: for scores up to 8 about
     sqrt(40) 2^-23 8 = 6e-6 a score, over at least five tokens of weight 2.7e-6, of an lse of 4 or more 7e-7.  1e-6 of
     itself is allowed (2-norm)."""
     rows, heads = 24, 64

@@ -1,6 +1,5 @@
 """The example decode step (examples/sparse_decode.py) as an MLA step: the latent normed, ropes rotated in both slot
-formats; the step repeats itself, eager and in a graph; the new
-token takes part with its own weight."""
+formats; the step repeats itself, eager and in a graph; the new token takes part with its own weight."""
 import numpy as np
 import pytest
 import torch
@@ -24,7 +23,8 @@ def test_latent_is_normed_and_ropes_are_rotated(hcu, dev, example, slots):  # no
     qr, kvr, per, _ = M.rope_qout_kv_store(t.positions.cpu().numpy(), q[..., 512:], kv, _u16(st["kv_weight"]), 1e-6, pe,
                                            _u16(st["cos_sin"]), False, np.zeros((1, 656), np.uint8), np.zeros(0, np.int64))
     got_q = _u16(st["q_cat"])
-    assert np.array_equal(got_q[..., 512:], qr.reshape(got_q[..., 512:].shape)) and np.array_equal(got_q[..., :512], q[..., :512])
+    assert np.array_equal(got_q[..., 512:], qr.reshape(got_q[..., 512:].shape))
+    assert np.array_equal(got_q[..., :512], q[..., :512])
     assert not np.array_equal(qr.reshape(-1), q[..., 512:].reshape(-1))
     normed = _u16(st["kv_c"])
     assert np.abs(normed.astype(np.int32) - kvr.astype(np.int32)).max() <= 1  # rsqrtf: one bf16 step
